@@ -23,17 +23,17 @@ __device__ unsigned long long g_trace[3 * 256 * 32];
 
 // Second profiling build (tools/trace2_build.py, -DCCSP_TRACE2; round 5): the phase boundaries of EVERY workgroup of k_rowgemm_h2 at the product
 // kernel's own residency (three workgroups per CU in MODE 0), with the hardware slot the workgroup ran on (HW_ID: shader engine, CU, SIMD of
-// wave 0; XCC_ID), so that the phases of the workgroups that SHARE a compute unit can be laid next to each other on that CU's own clock.  Stamps
-// go to LDS (one ds_write_b32 of lane 0, a dword each: the low half of s_memtime) and leave for global memory once, at the kernel's end.
+// wave 0; XCC_ID), so that the phases of the workgroups that SHARE a compute unit can be laid next to each other on that CU's own clock.  A stamp is the
+// low half of s_memtime, stored by lane 0 of wave 0 straight to global memory.
 #ifdef CCSP_TRACE2
 __device__ unsigned int g_trace2[4096 * 40];
-// (scalar stores: no vector register, no exec-mask change, nothing added to the kernel's 168-VGPR budget; s_dcache_wb at the end)
+// (plain vector stores: each takes a slot of the load / store counter behind the loads in flight, so a hand-counted wait that follows one
+// waits for at least what it waits for without it)
 #define CCSP_TRK2_DECL unsigned int* const trk2_ptr = g_trace2 + (size_t)(blockIdx.x < 4096 ? blockIdx.x : 4095) * 40;
 #define CCSP_TRK2(k)                                                                                                              \
     do {                                                                                                                          \
         const unsigned int lo_ = (unsigned int)__builtin_amdgcn_s_memtime();                                                      \
-        const unsigned int off_ = 4u * (unsigned int)(k);                                                                         \
-        asm volatile("s_store_dword %0, %1, %2 glc" :: "s"(lo_), "s"(trk2_ptr), "s"(off_) : "memory");                            \
+        if (threadIdx.x == 0) trk2_ptr[k] = lo_;                                                                                  \
     } while (0)
 #define CCSP_TRK2_FLUSH()                                                                                                         \
     do {                                                                                                                          \
@@ -41,11 +41,7 @@ __device__ unsigned int g_trace2[4096 * 40];
         asm volatile("s_getreg_b32 %0, hwreg(HW_REG_HW_ID)" : "=s"(h0_));                                                         \
         asm volatile("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(h1_));                                                        \
         const unsigned int rt_ = (unsigned int)__builtin_amdgcn_s_memrealtime();                                                  \
-        const unsigned int o0_ = 4u * 36u, o1_ = 4u * 37u, o2_ = 4u * 38u;                                                        \
-        asm volatile("s_store_dword %0, %1, %2 glc" :: "s"(h0_), "s"(trk2_ptr), "s"(o0_) : "memory");                             \
-        asm volatile("s_store_dword %0, %1, %2 glc" :: "s"(h1_), "s"(trk2_ptr), "s"(o1_) : "memory");                             \
-        asm volatile("s_store_dword %0, %1, %2 glc" :: "s"(rt_), "s"(trk2_ptr), "s"(o2_) : "memory");                             \
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");                                                        \
+        if (threadIdx.x == 0) { trk2_ptr[36] = h0_; trk2_ptr[37] = h1_; trk2_ptr[38] = rt_; }                                     \
     } while (0)
 #else
 #define CCSP_TRK2_DECL
