@@ -28,5 +28,6 @@ from .denoise_fn import ComposedEBMDenoiseFn, ConstraintDiffuser  # noqa: F401,E
 from .ddpm import GaussianDiffusion  # noqa: F401,E402
 
 from . import evaluate  # noqa: F401,E402
+from . import operators  # noqa: F401,E402
 
 __version__ = "0.1.0"

@@ -1,0 +1,90 @@
+/* ccsp_ops.h -- C ABI of the operator library (libccsp_ops.so): rows sorted by expert and combined back, the experts' products, the global
+ * gradient norm with clipping, each with its gradient.  diffusion-ccsp_amd/operators.py is the binding.
+ *
+ * The denoiser sends every edge of a constraint graph through the MLP of its constraint type and adds the results onto the edge's nodes
+ * with the weight 1 / sqrt(degree) (networks/denoise_fn.py:313-389, :508-523): a mixture of experts with a fixed router.  These
+ * operators are that in general form, for training (any types, widths, weights and routers) and for single tokens.
+ *
+ * Conventions
+ *  - every array pointer is a DEVICE pointer owned by the caller unless the parameter is documented "host"; rows are contiguous in their
+ *    last dimension, *_stride is the distance of two rows in ELEMENTS; an element pointer is aligned to its element, nothing more;
+ *  - every call enqueues its work on `stream` (hipStream_t as void*; NULL = the default stream) of the CURRENT device and returns: nothing here
+ *    allocates, synchronises or copies to the host, so every call may be captured into a graph;
+ *  - return value 0 = ok, non-zero = error; ccsp_ops_last_error() gives the thread-local message; no exception crosses the boundary;
+ *  - the library keeps no state between calls: calls on different streams, threads and devices are independent as long as their
+ *    buffers are;
+ *  - results do not depend on how blocks are scheduled: the same call on the same data gives the same bits. */
+#ifndef CCSP_OPS_H
+#define CCSP_OPS_H
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define CCSP_OPS_VERSION_MAJOR 1
+#define CCSP_OPS_VERSION_MINOR 0
+
+enum { CCSP_OPS_F32 = 0, CCSP_OPS_BF16 = 1, CCSP_OPS_F16 = 2 };
+enum { CCSP_OPS_NONE = 0, CCSP_OPS_SILU = 1 };
+
+#define CCSP_OPS_MAX_ASSIGN (1 << 30)     /* assignments, rows, tokens */
+#define CCSP_OPS_MAX_EXPERTS 1024
+#define CCSP_OPS_MAX_WIDTH (1 << 24)
+
+int32_t ccsp_ops_version(void);           /* major * 1000 + minor */
+const char* ccsp_ops_last_error(void);
+
+/* The plan of a routed layer.  Assignment a in [0, n_assign) joins expert[a] to token[a], or to token a / k where `token` is NULL (then n_assign =
+ * n_tokens * k).  Ids are signed whole numbers of id_bits (32 or 64) bits; an assignment with an id out of range is dropped.
+ *   offsets      [n_experts + 1]  first row of every expert; offsets[n_experts] = active rows
+ *   rows         [n_assign]       row of every assignment (by expert, then by assignment), -1 if dropped
+ *   assign       [n_assign]       assignment of every row; behind the last active row ~a of the dropped ones
+ *   row_token    [n_assign]       token of every row, -1 behind the last active row
+ *   token_ptr    [n_tokens + 1], token_assign [n_assign] (both or neither: token_ptr says that there is a list): the active assignments of every token, ascending
+ * workspace: ccsp_ops_route_workspace bytes (-1: an argument is out of range), free again when the call's work is done. */
+int64_t ccsp_ops_route_workspace(int64_t n_assign, int32_t n_experts, int64_t n_tokens, int32_t list_tokens);
+int ccsp_ops_route(const void* expert, const void* token, int32_t id_bits, int64_t n_assign, int32_t k, int32_t n_experts, int64_t n_tokens,
+                   int32_t* offsets, int32_t* rows, int32_t* assign, int32_t* row_token, int32_t* token_ptr, int32_t* token_assign,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dst[p] = src[row_token[p]] for p < n_rows, zeros where row_token[p] < 0.  dst [n_rows, width] contiguous. */
+int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void* src, int64_t src_stride, const int32_t* row_token, void* dst, void* stream);
+/* dst[n] = sum over the token's active assignments a, ascending, of weight[a] * src[rows[a]]; sums in 32 bits, rounded once.  token_ptr /
+ * token_assign NULL: assignments n k .. n k + k - 1.  weight NULL: 1; else of weight_type (32 bits or the rows' type).  A token without active assignments
+ * gets zeros.  dst [n_tokens, width] contiguous. */
+int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
+                          int32_t weight_type, const void* src, int64_t src_stride, void* dst, void* stream);
+/* Gradient of rows_combine: d_src[p] = weight[a] * dy[token], zeros behind the last active row; d_weight[a] = <dy[token], src[p]>, 0 for
+ * dropped assignments.  Either of d_src / d_weight may be NULL. */
+int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_t* assign, const int32_t* row_token, const void* weight, int32_t weight_type, const void* dy,
+                       int64_t dy_stride, const void* src, int64_t src_stride, void* d_src, void* d_weight, void* stream);
+
+/* The experts' products.  Rows offsets[e] .. offsets[e + 1] - 1 belong to expert e; weight [n_experts, out, inp] and bias [n_experts, out] (NULL: none) are
+ * contiguous.  y = act(x weight[e]^T + bias[e]) [n_rows, out] contiguous, zeros in the rows behind offsets[n_experts].  z, where not NULL, receives the
+ * pre-activation of the active rows (what silu_back reads).  Products and sums in 32 bits. */
+int ccsp_ops_linear(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* x, int64_t x_stride, const void* weight,
+                    const void* bias, int32_t activation, void* y, void* z, void* stream);
+/* dz = dy * silu'(z) in the active rows; the rows behind are not written. */
+int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, int64_t out, const int32_t* offsets, const void* dy, int64_t dy_stride, const void* z, void* dz,
+                              void* stream);
+/* dx = dz weight[e] [n_rows, inp], zeros behind the last active row. */
+int ccsp_ops_linear_back_input(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride,
+                               const void* weight, void* dx, void* stream);
+/* d_weight[e] = sum over the expert's rows of dz^T x, d_bias[e] = sum of dz; zeros for an expert without rows.  Either may be NULL. */
+int ccsp_ops_linear_back_weight(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride, const void* x,
+                                int64_t x_stride, void* d_weight, void* d_bias, void* stream);
+
+/* norm[0] = sqrt(sum of squares over all elements of all tensors), squares and sums in 64 bits.  in / out / sizes / types are HOST arrays of n_tensors entries
+ * (contiguous tensors, sizes in elements, types CCSP_OPS_*).  out not NULL: out[i] = in[i] * min(1, max_norm / (norm + 1e-6)), out[i] of the type of in[i], the same
+ * memory or disjoint; scale[0] receives the factor.  A norm that is not finite gives what the formula gives: an infinite one the factor 0, NaN NaN.
+ * norm, scale: one float each.  workspace: ccsp_ops_norm_workspace bytes. */
+int64_t ccsp_ops_norm_workspace(int32_t n_tensors, const int64_t* sizes);
+int ccsp_ops_clip_norm(int32_t n_tensors, const void* const* in, void* const* out, const int64_t* sizes, const int32_t* types, double max_norm, float* norm, float* scale,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

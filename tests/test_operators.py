@@ -1,0 +1,676 @@
+"""The operators of diffusion_ccsp_amd.operators (include/ccsp_ops.h) against plain 64-bit restatements on the CPU.
+
+Tolerances are bounds, worked out per element before the first run.  u(t) = finfo(t).eps / 2 is the relative error of one rounding to t.  A sum of n terms held in
+32 bits is off by at most 2 n u(fp32) times the sum of the terms' magnitudes in any order (the 2 allows a matrix instruction whose inner adds
+truncate); a result is rounded once to its type, plus half of that type's smallest step where it is subnormal."""
+import ctypes
+import math
+import os
+import re
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import ROOT
+from diffusion_ccsp_amd import CcspError, _ops
+from diffusion_ccsp_amd import operators as ops
+
+DTYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+U32 = 2.0 ** -24
+
+
+def u(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def tiny(dt):
+    """half the smallest step of the type"""
+    return torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2
+
+
+def close(got, want, bound, what):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape, what
+    bad = ~((got - want).abs() <= bound)
+    assert not bad.any(), '%s: %d of %d beyond the bound, worst %g over %g' % (
+        what, int(bad.sum()), bad.numel(), float((got - want).abs()[bad].max()), float(torch.as_tensor(bound).expand_as(want)[bad].max()))
+
+
+def plan_oracle(expert, E, token, N):
+    """assignments by (expert, assignment) and by (token, assignment), in plain Python order"""
+    e, t = expert.reshape(-1).tolist(), token.reshape(-1).tolist()
+    act = [0 <= x < E and 0 <= y < N for x, y in zip(e, t)]
+    by_expert = sorted((a for a in range(len(e)) if act[a]), key=lambda a: (e[a], a))
+    by_token = sorted((a for a in range(len(e)) if act[a]), key=lambda a: (t[a], a))
+    dropped = [a for a in range(len(e)) if not act[a]]
+    return e, t, by_expert, by_token, dropped
+
+
+def topk_tokens(expert):
+    k = 1 if expert.dim() == 1 else expert.shape[1]
+    return (torch.arange(expert.numel()) // max(k, 1)).reshape(expert.shape)
+
+
+# ---- without a GPU: the library, the refusals ----------------------------------------------------------------------------
+
+def test_library_exports_every_declared_symbol():
+    text = re.sub(r'/\*.*?\*/', '', open(os.path.join(ROOT, 'include', 'ccsp_ops.h')).read(), flags=re.S)
+    names = sorted(set(re.findall(r'\b(ccsp_ops_[a-z_0-9]+)\s*\(', text)))
+    L = _ops.lib()
+    assert len(names) == 13
+    for n in names:
+        assert hasattr(L, n), n
+    assert L.ccsp_ops_version() // 1000 == _ops.OPS_ABI_MAJOR
+
+
+def test_a_library_of_another_major_version_is_refused(monkeypatch):
+    monkeypatch.setattr(_ops, '_lib', None)
+    monkeypatch.setattr(_ops, 'OPS_ABI_MAJOR', _ops.OPS_ABI_MAJOR + 1)
+    with pytest.raises(CcspError, match='ABI version'):
+        _ops.lib()
+
+
+def test_c_entries_refuse_before_any_launch():
+    """every refusal below returns from the argument checks: no device is touched"""
+    L = _ops.lib()
+    ok = 64                                                       # (a non-null address that is never read)
+
+    def refused(rc, word):
+        assert rc != 0 and word in L.ccsp_ops_last_error().decode(), L.ccsp_ops_last_error()
+    refused(L.ccsp_ops_route(ok, None, 16, 4, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), '32 or 64')
+    refused(L.ccsp_ops_route(ok, None, 32, 5, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'tokens of 2 each')
+    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 0, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'experts')
+    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 1025, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'experts')
+    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 3, None), 'workspace')
+    refused(L.ccsp_ops_route(ok, ok, 32, 4, 0, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'token_ptr')
+    refused(L.ccsp_ops_route(None, None, 32, 4, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'null')
+    assert L.ccsp_ops_route_workspace(-1, 4, 4, 0) == -1 and L.ccsp_ops_route_workspace((1 << 30) + 1, 4, 4, 0) == -1
+    refused(L.ccsp_ops_rows_gather(7, 4, 4, ok, 4, ok, ok, None), 'type')
+    refused(L.ccsp_ops_rows_gather(0, 4, 4, ok, 4, None, ok, None), 'null')
+    refused(L.ccsp_ops_rows_gather(0, -1, 4, ok, 4, ok, ok, None), 'range')
+    refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, ok, 2, ok, 4, ok, None), 'weights')
+    refused(L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, 2, ok, 4, ok, 4, ok, ok, None), 'weights')
+    refused(L.ccsp_ops_linear(0, 4, 4, 0, 4, ok, ok, 4, ok, None, 0, ok, None, None), 'range')
+    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, ok, None, 5, ok, None, None), 'activation')
+    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, None, ok, 4, ok, None, 0, ok, None, None), 'null')
+    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, None, None, 0, ok, None, None), 'null')
+    refused(L.ccsp_ops_linear_back_input(0, 4, 4, 4, 4, ok, ok, 4, None, ok, None), 'null')
+    refused(L.ccsp_ops_linear_back_weight(0, 4, 4, 4, 4, ok, ok, 4, ok, 4, None, None, None), 'null')
+    refused(L.ccsp_ops_linear_silu_back(0, 4, 4, 4, ok, ok, 4, None, ok, None), 'null')
+    sizes, types, ptrs = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(0), (ctypes.c_void_p * 1)(64)
+    refused(L.ccsp_ops_clip_norm(1, ptrs, ptrs, sizes, types, -1.0, ok, ok, ok, 64, None), 'negative')
+    refused(L.ccsp_ops_clip_norm(1, ptrs, ptrs, sizes, types, 1.0, ok, None, ok, 64, None), 'factor')
+    refused(L.ccsp_ops_clip_norm(1, ptrs, None, sizes, types, 1.0, ok, ok, ok, 8, None), 'workspace')
+    types[0] = 9
+    refused(L.ccsp_ops_clip_norm(1, ptrs, None, sizes, types, 1.0, ok, ok, ok, 64, None), 'type')
+    assert L.ccsp_ops_norm_workspace(1, (ctypes.c_int64 * 1)(-4)) == -1
+
+
+def test_cpu_tensors_are_refused():
+    for call in (lambda: ops.route(torch.zeros(4, dtype=torch.int64), 2), lambda: ops.global_norm([torch.zeros(3)]),
+                 lambda: ops.clip_global_norm([torch.zeros(3)], 1.0)):
+        with pytest.raises(CcspError, match='no CPU fallback'):
+            call()
+    with pytest.raises(ValueError, match='no tensors'):
+        ops.global_norm([])
+    assert float(ops.clip_grad_norm_([torch.nn.Parameter(torch.zeros(2))], 1.0)) == 0.0
+
+
+# ---- routes --------------------------------------------------------------------------------------------------------------
+
+def ids(A, E, seed, drop, hot=False):
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(0, E, (A,), generator=g)
+    if hot:
+        e = torch.where(torch.rand(A, generator=g) < 0.9, torch.full_like(e, E // 2), e)
+    if drop:
+        far = torch.tensor([-1, E, E + 1000, -2 ** 31, 2 ** 31 - 1])
+        e = torch.where(torch.rand(A, generator=g) < drop, far[torch.randint(0, 5, (A,), generator=g)], e)
+    return e
+
+
+def check_plan(plan, expert, E, token, N, listed):
+    e, t, by_expert, by_token, dropped = plan_oracle(expert, E, token, N)
+    A, n = len(e), len(by_expert)
+    off, rows = plan.offsets.cpu().tolist(), plan.rows.cpu().tolist()
+    counts = np.bincount([e[a] for a in by_expert], minlength=E) if n else np.zeros(E, int)
+    assert off == [0] + np.cumsum(counts).tolist()
+    want = [-1] * A
+    for p, a in enumerate(by_expert):
+        want[a] = p
+    assert rows == want
+    assert plan.assign.cpu().tolist() == by_expert + [~a for a in dropped]
+    assert plan.row_token.cpu().tolist() == [t[a] for a in by_expert] + [-1] * (A - n)
+    assert plan.counts.cpu().tolist() == counts.tolist()
+    if listed:
+        ptr = plan.token_ptr.cpu().tolist()
+        per = np.bincount([t[a] for a in by_token], minlength=N) if n else np.zeros(N, int)
+        assert ptr == [0] + np.cumsum(per).tolist()
+        assert plan.token_assign.cpu().tolist()[:n] == by_token
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('A,E,drop,hot', [(1, 1, 0, False), (1, 64, 0, False), (63, 3, 0.2, False), (64, 13, 0, False), (65, 1024, 0.1, False), (2049, 13, 0.3, True), (8191, 1024, 0, False),
+                                          (8192, 7, 1.0, False), (8193, 7, 0.1, True), (40001, 1024, 0.2, False), (150000, 64, 0, True)])
+@pytest.mark.parametrize('bits', [32, 64])
+def test_route_top_k(device, A, E, drop, hot, bits):
+    expert = ids(A, E, A + E, drop, hot)
+    if bits == 64 and drop:
+        expert[::17] = 2 ** 40 + 1                                # (low half in range)
+    expert = expert.to(torch.int32 if bits == 32 else torch.int64)
+    for k in (1, 3):
+        ex = expert[:A - A % k].reshape(-1, k) if k > 1 else expert
+        if ex.numel() == 0:
+            continue
+        plan = ops.route(ex.to(device), E)
+        check_plan(plan, ex, E, topk_tokens(ex), ex.shape[0], False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('A,E,N,drop', [(1, 1, 1, 0), (5, 2, 3, 0.5), (700, 13, 90, 0.1), (8192, 13, 1023, 0), (8000, 13, 1024, 0), (8192, 40, 16384, 0.2), (500, 3, 16385, 0), (500, 3, 70000, 0.1),
+                                        (9001, 13, 4095, 0.1), (9001, 13, 4096, 0), (40528, 13, 2304, 0), (30000, 1024, 1, 0), (50000, 5, 300000, 0.3)])
+@pytest.mark.parametrize('bits', [32, 64])
+def test_route_listed_tokens(device, A, E, N, drop, bits):
+    dt = torch.int32 if bits == 32 else torch.int64
+    expert, token = ids(A, E, A, drop).to(dt), ids(A, N, A + 1, drop / 2).to(dt)
+    plan = ops.route(expert.to(device), E, tokens=token.to(device), n_tokens=N)
+    check_plan(plan, expert, E, token, N, True)
+
+
+@pytest.mark.gpu
+def test_route_of_nothing(device):
+    none = torch.zeros((0, 2), dtype=torch.int64, device=device)
+    plan = ops.route(none, 5)
+    assert plan.offsets.cpu().tolist() == [0] * 6 and plan.n_rows == 0 and plan.n_tokens == 0
+    plan = ops.route(none, 5, tokens=none, n_tokens=3)
+    assert plan.offsets.cpu().tolist() == [0] * 6 and plan.token_ptr.cpu().tolist() == [0] * 4
+    x = torch.randn(3, 4, device=device, requires_grad=True)
+    w = torch.randn(5, 6, 4, device=device, requires_grad=True)
+    b = torch.randn(5, 6, device=device, requires_grad=True)
+    xs = ops.sort_rows(x, plan)
+    y = ops.combine_rows(ops.expert_linear(xs, w, plan, b, 'silu'), plan)
+    assert tuple(xs.shape) == (0, 4) and torch.equal(y, torch.zeros(3, 6, device=device))
+    g = torch.autograd.grad(y.sum(), [x, w, b])
+    assert all(float(t.abs().max()) == 0.0 for t in g)
+
+
+@pytest.mark.gpu
+def test_route_refusals(device):
+    e = torch.zeros((4, 2), dtype=torch.int64, device=device)
+    with pytest.raises(TypeError, match='int32 or int64'):
+        ops.route(e.float(), 3)
+    with pytest.raises(ValueError, match='experts'):
+        ops.route(e, 0)
+    with pytest.raises(ValueError, match='experts'):
+        ops.route(e, 1025)
+    with pytest.raises(ValueError, match='N, k'):
+        ops.route(e[None], 3)
+    with pytest.raises(ValueError, match='5 tokens'):
+        ops.route(e, 3, n_tokens=5)
+    with pytest.raises(ValueError, match='n_tokens'):
+        ops.route(e, 3, tokens=e)
+    with pytest.raises(ValueError, match='differ'):
+        ops.route(e, 3, tokens=e.int(), n_tokens=4)
+    with pytest.raises(ValueError, match='no expert'):
+        ops.route(e[:, :0], 3)
+    plan = ops.route(e, 3)
+    x = torch.zeros(4, 5, device=device)
+    with pytest.raises(ValueError, match='one row per token'):
+        ops.sort_rows(x[:3], plan)
+    with pytest.raises(TypeError, match='float64'):
+        ops.sort_rows(x.double(), plan)
+    with pytest.raises(ValueError, match='one row per assignment'):
+        ops.combine_rows(x, plan)
+    ys = torch.zeros(8, 5, device=device)
+    with pytest.raises(ValueError, match='weights'):
+        ops.combine_rows(ys, plan, torch.zeros(8, device=device))
+    with pytest.raises(TypeError, match='weights'):
+        ops.combine_rows(ys, plan, torch.zeros(4, 2, device=device, dtype=torch.float16))
+    w = torch.zeros(3, 6, 5, device=device)
+    with pytest.raises(ValueError, match='weight must be'):
+        ops.expert_linear(ys, w[:2], plan)
+    with pytest.raises(ValueError, match='bias must be'):
+        ops.expert_linear(ys, w, plan, bias=w[:, :, 0].t())
+    with pytest.raises(TypeError, match='one type'):
+        ops.expert_linear(ys, w.half(), plan)
+    with pytest.raises(ValueError, match='activation'):
+        ops.expert_linear(ys, w, plan, activation='relu')
+    with pytest.raises(CcspError, match='no CPU fallback'):
+        ops.sort_rows(x.cpu(), plan)
+
+
+# ---- rows there and back -------------------------------------------------------------------------------------------------
+
+def strided(t, how, device):
+    """the same values in another memory layout: rows further apart than their width, starting off the allocation's alignment"""
+    t = t.to(device)
+    if how == 'plain':
+        return t
+    wide = torch.full((t.shape[0], t.shape[1] + 3), float('nan'), dtype=t.dtype, device=device)
+    wide[:, 1:1 + t.shape[1]] = t
+    if how == 'offset':
+        return wide[:, 1:1 + t.shape[1]]
+    return t.t().contiguous().t()                                 # 'columns': the last dimension is not contiguous
+
+
+ROWS = [(1, 1, 1, 1), (1, 8, 64, 40), (7, 3, 4, 5), (40, 2, 13, 4), (130, 4, 8, 72), (33, 1, 3, 1001), (257, 8, 16, 256), (19, 5, 1024, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('N,k,E,D', ROWS)
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('form', ['topk', 'listed'])
+@pytest.mark.parametrize('layout', ['plain', 'offset', 'columns'])
+def test_sort_and_combine_with_gradients(device, N, k, E, D, dtype, form, layout):
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(N * 1000 + D)
+    expert = ids(N * k, E, N + k, 0.25).reshape(N, k)
+    token = topk_tokens(expert) if form == 'topk' else ids(N * k, N, 3 * N, 0.1).reshape(N, k)
+    x, g_y = torch.randn(N, D, generator=g).to(dt), torch.randn(N, D, generator=g).to(dt)
+    ys, g_xs = torch.randn(N * k, D, generator=g).to(dt), torch.randn(N * k, D, generator=g).to(dt)
+    for wdt in (None, torch.float32, dt):
+        w = None if wdt is None else torch.randn(N, k, generator=g).to(wdt)
+        e, t, by_expert, by_token, dropped = plan_oracle(expert, E, token, N)
+        n = len(by_expert)
+        ys_, gxs_ = ys.clone(), g_xs.clone()
+        ys_[n:] = float('nan')                                    # what lies behind the last active row reaches nothing
+        gxs_[n:] = float('nan')
+        plan = ops.route(expert.to(device), E, **({} if form == 'topk' else dict(tokens=token.to(device), n_tokens=N)))
+        xd, yd = strided(x, layout, device).requires_grad_(), strided(ys_, layout, device).requires_grad_()
+        wd = None if w is None else w.to(device).requires_grad_()
+        xs = ops.sort_rows(xd, plan)
+        y = ops.combine_rows(yd, plan, wd)
+        wrt = [xd, yd] + ([] if wd is None else [wd])
+        grads = torch.autograd.grad([xs, y], wrt, [strided(gxs_, layout, device), strided(g_y, layout, device)])
+        tok = torch.tensor([t[a] for a in by_expert], dtype=torch.long)
+        X, YS, GY, GX = x.double(), ys.double(), g_y.double(), g_xs.double()
+        W = torch.ones(N * k, dtype=torch.float64) if w is None else w.double().reshape(-1)
+        wr = W[torch.tensor(by_expert, dtype=torch.long)][:, None]
+        want_xs = torch.zeros(N * k, D, dtype=torch.float64)
+        want_xs[:n] = X[tok]
+        assert torch.equal(xs.detach().cpu().double(), want_xs)
+        want_y, mag = torch.zeros(N, D, dtype=torch.float64), torch.zeros(N, D, dtype=torch.float64)
+        want_dx, mag_x = want_y.clone(), want_y.clone()
+        deg = torch.zeros(N, 1, dtype=torch.float64)
+        want_y.index_add_(0, tok, YS[:n] * wr)
+        mag.index_add_(0, tok, (YS[:n] * wr).abs())
+        want_dx.index_add_(0, tok, GX[:n])
+        mag_x.index_add_(0, tok, GX[:n].abs())
+        deg.index_add_(0, tok, torch.ones(n, 1, dtype=torch.float64))
+        close(y, want_y, u(dt) * want_y.abs() + 2 * (deg + 1) * U32 * mag + tiny(dt), 'y')
+        close(grads[0], want_dx, u(dt) * want_dx.abs() + 2 * (deg + 1) * U32 * mag_x + tiny(dt), 'd x')
+        want_dys = torch.zeros(N * k, D, dtype=torch.float64)
+        want_dys[:n] = GY[tok] * wr
+        close(grads[1], want_dys, (u(dt) + 2 * U32) * want_dys.abs() + tiny(dt), 'd ys')
+        if w is not None:
+            want_dw, mag_w = torch.zeros(N * k, dtype=torch.float64), torch.zeros(N * k, dtype=torch.float64)
+            at = torch.tensor(by_expert, dtype=torch.long)
+            want_dw[at], mag_w[at] = (GY[tok] * YS[:n]).sum(1), (GY[tok] * YS[:n]).abs().sum(1)
+            bound = u(wdt) * want_dw.abs() + 2 * D * U32 * mag_w + tiny(wdt)
+            close(grads[2].reshape(-1), want_dw, bound, 'd weights')
+
+
+@pytest.mark.gpu
+def test_rows_keep_infinities_and_nan_of_active_rows_only(device):
+    expert = torch.tensor([[0, 1], [1, -1], [-1, -1]])
+    plan = ops.route(expert.to(device), 2)
+    ys = torch.tensor([[1.0, float('inf')], [2.0, 3.0], [float('nan'), -float('inf')], [float('nan')] * 2, [float('nan')] * 2, [float('nan')] * 2], device=device)
+    w = torch.tensor([[1.0, 1.0], [1.0, float('nan')], [float('inf'), float('nan')]], device=device)
+    y = ops.combine_rows(ys, plan, w)                            # rows: (0, 0) -> 0, (0, 1) -> 1, (1, 0) -> 2
+    want = torch.tensor([[3.0, float('inf')], [float('nan'), -float('inf')], [0.0, 0.0]])
+    assert torch.equal(torch.nan_to_num(y.cpu(), nan=-7.0), torch.nan_to_num(want, nan=-7.0))
+
+
+# ---- products ------------------------------------------------------------------------------------------------------------
+
+def linear_case(counts, tail, I, O, dt, seed):
+    g = torch.Generator().manual_seed(seed)
+    R, E = sum(counts), len(counts)
+    expert = torch.cat([torch.full((n,), e) for e, n in enumerate(counts)] + [torch.full((tail,), -1)]).long()
+    b = 1.0 / math.sqrt(I)
+    xs, gy = torch.randn(R + tail, I, generator=g).to(dt), torch.randn(R + tail, O, generator=g).to(dt)
+    w, bias = ((torch.rand(E, O, I, generator=g) * 2 - 1) * b * 2).to(dt), (torch.rand(E, O, generator=g) * 2 - 1).to(dt)
+    return expert, xs, w, bias, gy
+
+
+def check_linear(device, counts, tail, I, O, dt, act, with_bias, layout='plain', seed=0):
+    expert, xs, w, bias, gy = linear_case(counts, tail, I, O, dt, seed)
+    R, E = sum(counts), len(counts)
+    xs_, gy_ = xs.clone(), gy.clone()
+    xs_[R:], gy_[R:] = float('nan'), float('nan')                # what lies behind the last group reaches nothing
+    plan = ops.route(expert.to(device), E)
+    xd, wd = strided(xs_, layout, device).requires_grad_(), w.to(device).requires_grad_()
+    bd = bias.to(device).requires_grad_() if with_bias else None
+    y = ops.expert_linear(xd, wd, plan, bd, act)
+    got = torch.autograd.grad(y, [t for t in (xd, wd, bd) if t is not None], strided(gy_, layout, device))
+    with torch.no_grad():
+        assert torch.equal(ops.expert_linear(xd, wd, plan, bd, act), y)          # (the form that keeps no pre-activation)
+    lo = 0
+    want_y, by = torch.zeros(R + tail, O, dtype=torch.float64), torch.zeros(R + tail, O, dtype=torch.float64)
+    want_x, bx = torch.zeros(R + tail, I, dtype=torch.float64), torch.zeros(R + tail, I, dtype=torch.float64)
+    want_w, bw = torch.zeros(E, O, I, dtype=torch.float64), torch.zeros(E, O, I, dtype=torch.float64)
+    want_b, bb = torch.zeros(E, O, dtype=torch.float64), torch.zeros(E, O, dtype=torch.float64)
+    for e, n in enumerate(counts):
+        s = slice(lo, lo + n)
+        lo += n
+        X, W, G = xs[s].double(), w[e].double(), gy[s].double()
+        z = X @ W.t() + (bias[e].double() if with_bias else 0.0)
+        ez = 2 * (I + 1) * U32 * (X.abs() @ W.abs().t() + (bias[e].double().abs() if with_bias else 0.0))
+        sg = torch.sigmoid(z)
+        if act:
+            # |silu'| <= 1.1, |silu''| <= 0.5; the exponential, sum and quotient of the sigmoid: a few units of 32 bits
+            want_y[s], by[s] = z * sg, 1.1 * ez + 8 * U32 * (z.abs() + 1) + u(dt) * (z * sg).abs() + tiny(dt)
+            slope = sg * (1 + z * (1 - sg))
+            dz = G * slope
+            # z is kept in the type: its rounding moves the slope by at most 0.5 u |z|; dz is rounded to the type
+            edz = G.abs() * (0.5 * (u(dt) * z.abs() + ez + tiny(dt)) + 16 * U32 * (z.abs() + 1)) + u(dt) * dz.abs() + tiny(dt)
+            edz = edz * (1 + u(dt))
+        else:
+            want_y[s], by[s] = z, ez + u(dt) * z.abs() + tiny(dt)
+            dz, edz = G, torch.zeros_like(G)
+        want_x[s] = dz @ W
+        bx[s] = edz @ W.abs() + 2 * (O + 1) * U32 * ((dz.abs() + edz) @ W.abs()) + u(dt) * (want_x[s].abs() + edz @ W.abs()) + tiny(dt)
+        want_w[e] = dz.t() @ X
+        bw[e] = edz.t() @ X.abs() + 2 * (n + 1) * U32 * ((dz.abs() + edz).t() @ X.abs()) + u(dt) * (want_w[e].abs() + edz.t() @ X.abs()) + tiny(dt)
+        want_b[e] = dz.sum(0)
+        bb[e] = edz.sum(0) + 2 * (n + 1) * U32 * (dz.abs() + edz).sum(0) + u(dt) * (want_b[e].abs() + edz.sum(0)) + tiny(dt)
+    close(y, want_y, by, 'y')
+    close(got[0], want_x, bx, 'd xs')
+    close(got[1], want_w, bw, 'd weight')
+    if with_bias:
+        close(got[2], want_b, bb, 'd bias')
+
+
+LINEAR = [([1], 0, 1, 1), ([0, 3, 0], 1, 8, 8), ([1, 1, 1, 1], 0, 64, 40), ([5, 0, 130], 3, 64, 128), ([127, 129, 1], 0, 72, 136), ([40, 17, 200], 5, 33, 65), ([300, 0, 0, 21], 0, 256, 264),
+          ([128, 256], 128, 128, 256), ([64, 70], 2, 13, 300), ([2, 0, 1], 0, 520, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('counts,tail,I,O', LINEAR)
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('act,with_bias', [(None, False), (None, True), ('silu', True), ('silu', False)])
+def test_expert_linear_with_gradients(device, counts, tail, I, O, dtype, act, with_bias):
+    check_linear(device, counts, tail, I, O, DTYPES[dtype], act, with_bias, seed=I + O)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('layout', ['offset', 'columns'])
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_expert_linear_on_strided_rows(device, layout, dtype):
+    check_linear(device, [70, 3, 150], 4, 64, 96, DTYPES[dtype], 'silu', True, layout=layout)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_expert_linear_of_many_experts(device, dtype):
+    """more experts than a wave has lanes, most of them empty; a long group that ends inside a tile"""
+    counts = [(3 * e) % 5 if e % 7 else 0 for e in range(201)]
+    counts[150] = 700
+    check_linear(device, counts, 9, 48, 56, DTYPES[dtype], None, True)
+
+
+@pytest.mark.gpu
+def test_expert_linear_gradient_against_differences(device):
+    """32-bit gradients against central differences of the 64-bit formula in random directions: the oracle's gradient is not taken on trust"""
+    counts, I, O = [5, 0, 9], 12, 10
+    expert, xs, w, bias, gy = linear_case(counts, 0, I, O, torch.float32, 3)
+    plan = ops.route(expert.to(device), 3)
+    leaves = [t.to(device).requires_grad_() for t in (xs, w, bias)]
+    grads = torch.autograd.grad(ops.expert_linear(leaves[0], leaves[1], plan, leaves[2], 'silu'), leaves, gy.to(device))
+
+    def f(x, W, b):
+        z = torch.cat([x[:5] @ W[0].t() + b[0], x[5:] @ W[2].t() + b[2]])
+        return float((z * torch.sigmoid(z) * gy.double()).sum())
+    at = [t.double() for t in (xs, w, bias)]
+    g = torch.Generator().manual_seed(1)
+    for i in range(3):
+        d = torch.randn(at[i].shape, generator=g, dtype=torch.float64)
+        h = 1e-5
+        up, dn = list(at), list(at)
+        up[i], dn[i] = at[i] + h * d, at[i] - h * d
+        num = (f(*up) - f(*dn)) / (2 * h)
+        got = float((grads[i].cpu().double() * d).sum())
+        # the difference quotient: h^2 / 6 times a third derivative of a few hundred, and the cancellation 1e-16 |f| / h
+        assert abs(got - num) <= 1e-4 * float((grads[i].cpu().double() * d).abs().sum()) + 1e-6, i
+
+
+@pytest.mark.gpu
+def test_a_frozen_weight_or_input_gets_no_gradient(device):
+    expert, xs, w, bias, gy = linear_case([4, 6], 0, 16, 24, torch.float32, 5)
+    plan = ops.route(expert.to(device), 2)
+    full = [t.to(device).requires_grad_() for t in (xs, w, bias)]
+    want = torch.autograd.grad(ops.expert_linear(full[0], full[1], plan, full[2], 'silu'), full, gy.to(device))
+    for i in range(3):
+        part = [t.to(device).requires_grad_(j == i) for j, t in enumerate((xs, w, bias))]
+        got = torch.autograd.grad(ops.expert_linear(part[0], part[1], plan, part[2], 'silu'), part[i], gy.to(device))[0]
+        assert torch.equal(got, want[i])
+
+
+# ---- the global norm -----------------------------------------------------------------------------------------------------
+
+def norm_oracle(ts, max_norm):
+    n = math.sqrt(sum(float((t.double() ** 2).sum()) for t in ts))
+    return n, min(1.0, max_norm / (n + 1e-6))
+
+
+def check_clip(got_norm, got, ts, max_norm):
+    n, c = norm_oracle(ts, max_norm)
+    assert abs(float(got_norm) - n) <= 2 * U32 * n               # one rounding to 32 bits, and 64-bit sums
+    for i, (a, t) in enumerate(zip(got, ts)):
+        want = t.double() * c
+        close(a, want, (u(t.dtype) + 4 * U32) * want.abs() + tiny(t.dtype), 'tensor %d' % i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES) + ['mixed'])
+@pytest.mark.parametrize('max_norm', [0.0, 0.7, 1e9, math.inf])
+def test_clip_global_norm(device, dtype, max_norm):
+    g = torch.Generator().manual_seed(5)
+    sizes = [(1,), (0,), (3, 5), (16384,), (16385,), (0, 7), (7,), (100003,), (2, 3, 4), (40000,)]
+    dts = list(DTYPES.values())
+    ts = [(torch.randn(s, generator=g) * 10.0 ** (i % 3 - 1)).to(dts[i % 3] if dtype == 'mixed' else DTYPES[dtype]) for i, s in enumerate(sizes)]
+    dev = [t.to(device) for t in ts]
+    assert abs(float(ops.global_norm(dev)) - norm_oracle(ts, 1.0)[0]) <= 2 * U32 * norm_oracle(ts, 1.0)[0]
+    out = [torch.full_like(t, 7.0) for t in dev]
+    check_clip(ops.clip_global_norm(dev, max_norm, out=out), out, ts, max_norm)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, ts))
+    check_clip(ops.clip_global_norm(dev, max_norm), dev, ts, max_norm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_clip_of_many_unaligned_tensors(device, dtype):
+    """more tensors than a launch's table holds, each starting anywhere in one buffer; the gaps between them stay"""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(2)
+    sizes = [int(v) for v in torch.randint(0, 90, (450,), generator=g)]
+    host = torch.randn(sum(sizes) + len(sizes), generator=g).to(dt)
+    buf, out = host.to(device), torch.full((sum(sizes) + 2 * len(sizes),), 7.0, dtype=dt, device=device)
+    src, dst, cpu, at, ot = [], [], [], 0, 0
+    for i, n in enumerate(sizes):
+        src.append(buf[at:at + n]); cpu.append(host[at:at + n]); dst.append(out[ot:ot + n])
+        at += n + i % 2
+        ot += n + i % 3
+    check_clip(ops.clip_global_norm(src, 2.5, out=dst), dst, cpu, 2.5)
+    assert torch.equal(buf.cpu(), host)
+    keep = torch.ones(out.numel(), dtype=torch.bool)
+    ot = 0
+    for i, n in enumerate(sizes):
+        keep[ot:ot + n] = False
+        ot += n + i % 3
+    assert bool((out.cpu()[keep] == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_norm_range_and_values_that_are_not_finite(device):
+    big = torch.full((1000,), 1e30, device=device)
+    assert abs(float(ops.global_norm([big])) / (1e30 * math.sqrt(1000.0)) - 1) < 1e-6
+    small = torch.full((1000,), 1e-30, device=device)
+    assert abs(float(ops.global_norm([small])) / (1e-30 * math.sqrt(1000.0)) - 1) < 1e-6
+    zero = torch.zeros(5, device=device)
+    assert float(ops.clip_global_norm([zero], 1.0)) == 0.0 and float(zero.abs().max()) == 0.0
+    a = torch.tensor([1.0, math.inf], device=device)
+    assert math.isinf(float(ops.clip_global_norm([a], 1.0)))
+    assert float(a[0]) == 0.0 and math.isnan(float(a[1]))
+    b = torch.tensor([1.0, math.nan], device=device)
+    assert math.isnan(float(ops.clip_global_norm([b], 1.0))) and bool(torch.isnan(b).all())
+
+
+@pytest.mark.gpu
+def test_clip_grad_norm_of_parameters(device):
+    g = torch.Generator().manual_seed(9)
+    ps = [torch.nn.Parameter(torch.zeros(6, 10, device=device)) for _ in range(3)] + [torch.nn.Parameter(torch.zeros(2, device=device))]
+    host = [torch.randn(6, 10, generator=g) for _ in range(3)]
+    for p, h in zip(ps, host):
+        p.grad = h.to(device)
+    ps[1].grad = host[1].to(device).t().contiguous().t()         # a gradient with another memory order
+    v = ps[0].grad._version
+    norm = ops.clip_grad_norm_(iter(ps + [ps[0]]), 0.5)          # without a gradient: skipped; twice: once
+    check_clip(norm, [p.grad for p in ps[:3]], host, 0.5)
+    assert ps[0].grad._version > v and ps[3].grad is None
+    with pytest.raises(ValueError, match='twice'):
+        ops.clip_global_norm([ps[0].grad, ps[0].grad], 1.0)
+    with pytest.raises(ValueError, match='negative'):
+        ops.clip_global_norm([ps[0].grad], -1.0)
+    with pytest.raises(ValueError, match='negative'):
+        ops.clip_global_norm([ps[0].grad], math.nan)
+    with pytest.raises(ValueError, match='same type and shape'):
+        ops.clip_global_norm([ps[0].grad], 1.0, out=[ps[0].grad[:2]])
+    with pytest.raises(TypeError, match='float64'):
+        ops.global_norm([ps[0].grad.double()])
+    with pytest.raises(TypeError, match='sparse'):
+        ops.global_norm([ps[0].grad.to_sparse()])
+
+
+# ---- together, as they are used ------------------------------------------------------------------------------------------
+
+def layer(x, plan, w1, b1, w2, weights):
+    h = ops.expert_linear(ops.sort_rows(x, plan), w1, plan, b1, 'silu')
+    return ops.combine_rows(ops.expert_linear(h, w2, plan), plan, weights)
+
+
+def layer_inputs(device, dt, N=50, k=2, E=6, D=32, H=48, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    expert = ids(N * k, E, seed, 0.1).reshape(N, k).to(device)
+    mk = lambda *s: (torch.randn(*s, generator=g) / math.sqrt(s[-1])).to(device, dt)     # noqa: E731
+    return expert, [mk(N, D), mk(E, H, D), mk(E, H), mk(E, D, H), torch.rand(N, k, generator=g).to(device)], E
+
+
+@pytest.mark.gpu
+def test_a_routed_layer_trains_like_its_plain_form(device):
+    """route, sort, two products, combine, backward, clip against torch's 64-bit autograd of the same layer.  Each of the six operators in a row adds at most some
+    (width + 2) units of 32 bits of its terms' magnitude: 1e-4 of the largest entry leaves an order of magnitude"""
+    expert, leaves, E = layer_inputs(device, torch.float32)
+    for t in leaves:
+        t.requires_grad_()
+    plan = ops.route(expert, E)
+    y = layer(leaves[0], plan, *leaves[1:])
+    y.square().sum().backward()
+    ref = [t.detach().cpu().double().requires_grad_() for t in leaves]
+    x, w1, b1, w2, wt = ref
+    want = torch.zeros(x.shape[0], w2.shape[1], dtype=torch.float64)
+    rows = []
+    for n in range(expert.shape[0]):
+        acc = torch.zeros(w2.shape[1], dtype=torch.float64)
+        for j in range(expert.shape[1]):
+            e = int(expert[n, j])
+            if 0 <= e < E:
+                acc = acc + wt[n, j] * (w2[e] @ torch.nn.functional.silu(w1[e] @ x[n] + b1[e]))
+        rows.append(acc)
+    want = torch.stack(rows)
+    want.square().sum().backward()
+    assert float((y.detach().cpu().double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    for t, r in zip(leaves, ref):
+        assert float((t.grad.cpu().double() - r.grad).abs().max()) <= 1e-4 * float(r.grad.abs().max())
+    norm = ops.clip_grad_norm_(leaves, 0.1)
+    want_norm = math.sqrt(sum(float((r.grad ** 2).sum()) for r in ref))
+    assert abs(float(norm) - want_norm) <= 1e-4 * want_norm
+    assert abs(float(ops.global_norm([t.grad for t in leaves])) - 0.1) <= 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_the_same_bits_every_time_and_on_any_stream(device, dtype):
+    expert, leaves, E = layer_inputs(device, DTYPES[dtype], N=700, k=4, E=13, D=64, H=96)
+
+    def once():
+        ls = [t.detach().clone().requires_grad_() for t in leaves]
+        plan = ops.route(expert, E)
+        y = layer(ls[0], plan, *ls[1:])
+        return [y.detach()] + list(torch.autograd.grad(y, ls, torch.ones_like(y)))
+    want = once()
+    torch.cuda.synchronize()
+    results = {}
+
+    def worker(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            results[i] = [once() for _ in range(3)]
+        s.synchronize()
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        for got in results[i]:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed(device):
+    """forward, backward and clipping in one graph; every replay, on new inputs and with eager work between, equals the eager result"""
+    expert, leaves, E = layer_inputs(device, torch.float32, N=300, k=3, E=7, D=40, H=56)
+    static = [t.clone().requires_grad_() for t in leaves]
+    ids_in = expert.clone()
+
+    def step():
+        plan = ops.route(ids_in, E)
+        y = layer(static[0], plan, *static[1:])
+        grads = torch.autograd.grad(y, static, torch.ones_like(y))
+        out = [torch.empty_like(t) for t in grads]
+        norm = ops.clip_global_norm(grads, 0.25, out=out)
+        return [plan.offsets, y, norm] + out
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(4):
+        ex, new, _ = layer_inputs(device, torch.float32, N=300, k=3, E=7, D=40, H=56, seed=seed + 10)
+        with torch.no_grad():
+            ids_in.copy_(ex)
+            for s, t in zip(static, new):
+                s.copy_(t)
+        graph.replay()
+        got = [t.detach().clone() for t in captured]
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
+
+
+@pytest.mark.gpu
+def test_two_graphs_do_not_share_workspaces(device):
+    """two captured routes replayed on two streams at once: each has its own memory"""
+    graphs = []
+    for seed in range(2):
+        expert = ids(30000, 20, seed, 0.1).to(device)
+        ops.route(expert, 20)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            plan = ops.route(expert, 20)
+        graphs.append((g, plan, ops.route(expert, 20), torch.cuda.Stream(), expert))    # (a graph reads its inputs where they were: they live on)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, _, _, s, _ in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for _, plan, want, _, _ in graphs:
+            assert torch.equal(plan.rows, want.rows) and torch.equal(plan.assign, want.assign) and torch.equal(plan.offsets, want.offsets)
