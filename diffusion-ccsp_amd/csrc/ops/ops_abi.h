@@ -85,7 +85,7 @@ int ccsp_ops_linear(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp
     CCSP_OPS_CHECK(x && weight && y, "linear: null argument");
     ProdArgs p = {};
     p.a = x; p.lda = x_stride; p.b = weight; p.ldb = inp; p.b_expert = inp * out; p.bias = bias; p.c = y; p.ldc = out; p.z = z;
-    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.N = (int)out; p.K = (int)inp; p.silu = activation == CCSP_OPS_SILU;
+    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.seg_log2 = 31; p.N = (int)out; p.K = (int)inp; p.silu = activation == CCSP_OPS_SILU;
     return dispatch_type(type, [&](auto t) { return launch_prod<decltype(t), PROD_FORWARD>(p, (hipStream_t)stream); });
 }
 
@@ -113,25 +113,38 @@ int ccsp_ops_linear_back_input(int32_t type, int32_t n_experts, int64_t n_rows, 
     CCSP_OPS_CHECK(dz && weight && dx, "linear_back_input: null argument");
     ProdArgs p = {};
     p.a = dz; p.lda = dz_stride; p.b = weight; p.ldb = inp; p.b_expert = inp * out; p.c = dx; p.ldc = inp;
-    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.N = (int)inp; p.K = (int)out;
+    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.seg_log2 = 31; p.N = (int)inp; p.K = (int)out;
     return dispatch_type(type, [&](auto t) { return launch_prod<decltype(t), PROD_INPUT>(p, (hipStream_t)stream); });
 }
 
+int64_t ccsp_ops_linear_back_weight_workspace(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out) {
+    if (!type_ok(type) || n_experts < 1 || n_experts > CCSP_OPS_MAX_EXPERTS || n_rows < 0 || n_rows > CCSP_OPS_MAX_ASSIGN || inp < 1 || inp > CCSP_OPS_MAX_WIDTH || out < 1 || out > CCSP_OPS_MAX_WIDTH) return -1;
+    int64_t slots = 0;
+    dispatch_type(type, [&](auto t) {
+        const int l = seg_log2_for<decltype(t)>(n_rows, n_experts, out, inp);
+        slots = l == 31 ? 0 : 2 * ((n_rows >> l) + 1);
+        return 0;
+    });
+    return slots * (out * inp + out) * 4;
+}
+
 int ccsp_ops_linear_back_weight(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride, const void* x, int64_t x_stride,
-                                void* d_weight, void* d_bias, void* stream) {
+                                void* d_weight, void* d_bias, void* workspace, int64_t workspace_bytes, void* stream) {
     if (check_linear("linear_back_weight", type, n_experts, n_rows, inp, out, offsets)) return 1;
-    CCSP_OPS_CHECK((n_rows == 0 || (dz && (x || !d_weight))) && (d_weight || d_bias), "linear_back_weight: null argument");
+    CCSP_OPS_CHECK((n_rows == 0 || (dz && x)) && (d_weight || d_bias), "linear_back_weight: null argument");
+    const int64_t need = ccsp_ops_linear_back_weight_workspace(type, n_experts, n_rows, inp, out);
+    CCSP_OPS_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "linear_back_weight: workspace of %lld bytes is too small or not aligned to 16 bytes",
+                   (long long)workspace_bytes);
     ProdArgs p = {};
     p.a = dz; p.lda = dz_stride; p.b = x; p.ldb = x_stride; p.c = d_weight; p.ldc = inp; p.c_expert = inp * out;
     p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = (int)out; p.N = (int)inp; p.K = -1;
+    p.sum = d_bias;                                              // (one kernel makes both; for the bias alone it goes over the first columns of x and writes no product)
+    p.parts = static_cast<float*>(workspace);
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;
-        if (d_weight && launch_prod<T, PROD_WEIGHT>(p, (hipStream_t)stream)) return 1;
-        if (d_bias) {
-            hipLaunchKernelGGL(k_bias_back<T>, dim3((unsigned)cdiv(out, 64), n_experts), dim3(256), 0, (hipStream_t)stream, offsets, (int)out, (const T*)dz, (long)dz_stride, (T*)d_bias);
-            LAUNCHED();
-        }
-        return 0;
+        p.seg_log2 = prod_direct<T, PROD_WEIGHT>(p) ? seg_log2_for<T>(n_rows, n_experts, out, inp) : 31;
+        if (!d_weight) p.N = p.N < 64 ? p.N : 64;
+        return launch_prod<T, PROD_WEIGHT>(p, (hipStream_t)stream);
     });
 }
 

@@ -209,7 +209,7 @@ class _ExpertLinear(Function):
         _run(x.device, _ops.lib().ccsp_ops_linear, _TYPE[x.dtype], E, plan.n_rows, I, O, plan.offsets.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(),
              None if bias is None else bias.data_ptr(), act, y.data_ptr(), None if z is None else z.data_ptr())
         ctx.plan, ctx.act = plan, act
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight, z)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None, weight, z)
         return y
 
     @staticmethod
@@ -234,8 +234,10 @@ class _ExpertLinear(Function):
                 d_w = torch.empty((E, O, I), dtype=g.dtype, device=dev)
             if ctx.needs_input_grad[2]:
                 d_b = torch.empty((E, O), dtype=g.dtype, device=dev)
-            _run(dev, L.ccsp_ops_linear_back_weight, code, E, plan.n_rows, I, O, off, dz.data_ptr(), dz.stride(0), x.data_ptr() if d_w is not None else None,
-                 x.stride(0) if d_w is not None else 0, None if d_w is None else d_w.data_ptr(), None if d_b is None else d_b.data_ptr())
+            need = L.ccsp_ops_linear_back_weight_workspace(code, E, plan.n_rows, I, O)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            _run(dev, L.ccsp_ops_linear_back_weight, code, E, plan.n_rows, I, O, off, dz.data_ptr(), dz.stride(0), x.data_ptr(), x.stride(0),
+                 None if d_w is None else d_w.data_ptr(), None if d_b is None else d_b.data_ptr(), ws.data_ptr(), need)
         return d_x, d_w, d_b, None, None
 
 

@@ -72,9 +72,11 @@ int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, i
 /* dx = dz weight[e] [n_rows, inp], zeros behind the last active row. */
 int ccsp_ops_linear_back_input(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride,
                                const void* weight, void* dx, void* stream);
-/* d_weight[e] = sum over the expert's rows of dz^T x, d_bias[e] = sum of dz; zeros for an expert without rows.  Either may be NULL. */
+/* d_weight[e] = sum over the expert's rows of dz^T x, d_bias[e] = sum of dz; zeros for an expert without rows.  Either may be
+ * NULL; d_bias has the same bits with and without d_weight.  workspace: ccsp_ops_linear_back_weight_workspace bytes (may be 0), aligned to 16. */
+int64_t ccsp_ops_linear_back_weight_workspace(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out);
 int ccsp_ops_linear_back_weight(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride, const void* x,
-                                int64_t x_stride, void* d_weight, void* d_bias, void* stream);
+                                int64_t x_stride, void* d_weight, void* d_bias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* norm[0] = sqrt(sum of squares over all elements of all tensors), squares and sums in 64 bits.  in / out / sizes / types are HOST arrays of n_tensors entries
  * (contiguous tensors, sizes in elements, types CCSP_OPS_*).  out not NULL: out[i] = in[i] * min(1, max_norm / (norm + 1e-6)), out[i] of the type of in[i], the same

@@ -59,7 +59,7 @@ def test_library_exports_every_declared_symbol():
     text = re.sub(r'/\*.*?\*/', '', open(os.path.join(ROOT, 'include', 'ccsp_ops.h')).read(), flags=re.S)
     names = sorted(set(re.findall(r'\b(ccsp_ops_[a-z_0-9]+)\s*\(', text)))
     L = _ops.lib()
-    assert len(names) == 13
+    assert len(names) == 14
     for n in names:
         assert hasattr(L, n), n
     assert L.ccsp_ops_version() // 1000 == _ops.OPS_ABI_MAJOR
@@ -97,7 +97,9 @@ def test_c_entries_refuse_before_any_launch():
     refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, None, ok, 4, ok, None, 0, ok, None, None), 'null')
     refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, None, None, 0, ok, None, None), 'null')
     refused(L.ccsp_ops_linear_back_input(0, 4, 4, 4, 4, ok, ok, 4, None, ok, None), 'null')
-    refused(L.ccsp_ops_linear_back_weight(0, 4, 4, 4, 4, ok, ok, 4, ok, 4, None, None, None), 'null')
+    refused(L.ccsp_ops_linear_back_weight(0, 4, 4, 4, 4, ok, ok, 4, ok, 4, None, None, ok, 64, None), 'null')
+    refused(L.ccsp_ops_linear_back_weight(0, 2, 2000, 4, 4, ok, ok, 4, ok, 4, ok, None, ok, 64, None), 'workspace')
+    assert L.ccsp_ops_linear_back_weight_workspace(0, 2, 2000, 0, 4) == -1
     refused(L.ccsp_ops_linear_silu_back(0, 4, 4, 4, ok, ok, 4, None, ok, None), 'null')
     sizes, types, ptrs = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(0), (ctypes.c_void_p * 1)(64)
     refused(L.ccsp_ops_clip_norm(1, ptrs, ptrs, sizes, types, -1.0, ok, ok, ok, 64, None), 'negative')
@@ -412,6 +414,31 @@ def test_expert_linear_of_many_experts(device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('counts', [[3000], [700, 1, 0, 1025, 512, 513], [2048, 1024, 1023, 4097, 0, 5], [1024, 1025, 1024, 1]])
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_expert_linear_with_rows_cut_into_segments(device, counts, dtype):
+    """experts longer than a segment of the weight gradient, at its border, and without rows beside them"""
+    need = _ops.lib().ccsp_ops_linear_back_weight_workspace(_ops.TYPES[str(DTYPES[dtype])[6:]], len(counts), sum(counts), 24, 40)
+    assert need > 0
+    check_linear(device, counts, 3, 24, 40, DTYPES[dtype], 'silu', True)
+    check_linear(device, counts, 0, 23, 41, DTYPES[dtype], None, True)
+
+
+def test_segments_of_cut_experts_have_slots_of_their_own():
+    """the slot rule of the weight gradient's partial sums (csrc/ops/ops_linear.h seg_slot), restated: no two share one, all lie in the workspace"""
+    rng = np.random.default_rng(0)
+    for _ in range(2000):
+        l = int(rng.integers(1, 6))
+        counts = rng.integers(0, int(rng.integers(1, 4 << l)) + 1, size=int(rng.integers(1, 12)))
+        off = np.concatenate([[0], np.cumsum(counts)])
+        used = []
+        for e, n in enumerate(counts):
+            if n > 1 << l:
+                used += [2 * ((int(off[e]) >> l) + i) + (i > 0) for i in range((int(n) + (1 << l) - 1) >> l)]
+        assert len(set(used)) == len(used) and all(0 <= s < 2 * ((int(off[-1]) >> l) + 1) for s in used), (l, counts)
+
+
+@pytest.mark.gpu
 def test_expert_linear_gradient_against_differences(device):
     """32-bit gradients against central differences of the 64-bit formula in random directions: the oracle's gradient is not taken on trust"""
     counts, I, O = [5, 0, 9], 12, 10
@@ -581,7 +608,7 @@ def test_a_routed_layer_trains_like_its_plain_form(device):
         rows.append(acc)
     want = torch.stack(rows)
     want.square().sum().backward()
-    assert float((y.detach().cpu().double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    assert float((y.detach().cpu().double() - want).abs().max()) <= 1e-4 * float(want.detach().abs().max())
     for t, r in zip(leaves, ref):
         assert float((t.grad.cpu().double() - r.grad).abs().max()) <= 1e-4 * float(r.grad.abs().max())
     norm = ops.clip_grad_norm_(leaves, 0.1)
