@@ -66,11 +66,11 @@ def lib():
     L.ccsp_ops_rows_gather.argtypes = [i32, i64, i64, vp, i64, vp, vp, vp]
     L.ccsp_ops_rows_combine.argtypes = [i32, i64, i64, i32, vp, vp, vp, vp, i32, vp, i64, vp, vp]
     L.ccsp_ops_rows_back.argtypes = [i32, i64, i64, vp, vp, vp, i32, vp, i64, vp, i64, vp, vp, vp]
-    L.ccsp_ops_linear.argtypes = [i32, i32, i64, i64, i64, vp, vp, i64, vp, vp, i32, vp, vp, vp]
+    L.ccsp_ops_linear_workspace.argtypes = [i32, i32, i32, i64, i64, i64, vp, i64, vp, i64]
+    L.ccsp_ops_linear_workspace.restype = i64
+    L.ccsp_ops_linear.argtypes = [i32, i32, i64, i64, i64, vp, vp, i64, vp, vp, i32, vp, vp, vp, i64, vp]
     L.ccsp_ops_linear_silu_back.argtypes = [i32, i32, i64, i64, vp, vp, i64, vp, vp, vp]
-    L.ccsp_ops_linear_back_input.argtypes = [i32, i32, i64, i64, i64, vp, vp, i64, vp, vp, vp]
-    L.ccsp_ops_linear_back_weight_workspace.argtypes = [i32, i32, i64, i64, i64]
-    L.ccsp_ops_linear_back_weight_workspace.restype = i64
+    L.ccsp_ops_linear_back_input.argtypes = [i32, i32, i64, i64, i64, vp, vp, i64, vp, vp, vp, i64, vp]
     L.ccsp_ops_linear_back_weight.argtypes = [i32, i32, i64, i64, i64, vp, vp, i64, vp, i64, vp, vp, vp, i64, vp]
     L.ccsp_ops_norm_workspace.argtypes = [i32, vp]
     L.ccsp_ops_norm_workspace.restype = i64

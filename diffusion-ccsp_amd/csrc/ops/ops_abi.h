@@ -5,8 +5,6 @@
 int32_t ccsp_ops_version(void) { return 1000 * CCSP_OPS_VERSION_MAJOR + CCSP_OPS_VERSION_MINOR; }
 const char* ccsp_ops_last_error(void) { return g_err; }
 
-#define CCSP_OPS_CHECK(cond, ...) do { if (!(cond)) return fail(__VA_ARGS__); } while (0)
-
 int64_t ccsp_ops_route_workspace(int64_t n_assign, int32_t n_experts, int64_t n_tokens, int32_t list_tokens) {
     if (n_assign < 0 || n_assign > CCSP_OPS_MAX_ASSIGN || n_experts < 1 || n_experts > CCSP_OPS_MAX_EXPERTS || n_tokens < 0 || n_tokens > CCSP_OPS_MAX_ASSIGN) return -1;
     return 4 * (int64_t)route_workspace_ints(n_assign, n_experts, n_tokens, list_tokens != 0);
@@ -71,22 +69,30 @@ int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_
 static int check_linear(const char* who, int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets) {
     CCSP_OPS_CHECK(type_ok(type), "%s: element type %d", who, type);
     CCSP_OPS_CHECK(n_experts >= 1 && n_experts <= CCSP_OPS_MAX_EXPERTS, "%s: %d experts, supported are 1 to %d", who, n_experts, CCSP_OPS_MAX_EXPERTS);
-    CCSP_OPS_CHECK(n_rows >= 0 && n_rows <= CCSP_OPS_MAX_ASSIGN && inp >= 1 && inp <= CCSP_OPS_MAX_WIDTH && out >= 1 && out <= CCSP_OPS_MAX_WIDTH,
+    CCSP_OPS_CHECK(n_rows >= 0 && n_rows <= CCSP_OPS_MAX_ASSIGN && inp >= 1 && inp <= CCSP_OPS_MAX_FEATURES && out >= 1 && out <= CCSP_OPS_MAX_FEATURES,
                    "%s: %lld rows, %lld -> %lld out of range", who, (long long)n_rows, (long long)inp, (long long)out);
     CCSP_OPS_CHECK(offsets, "%s: null argument", who);
     return 0;
 }
 
+int64_t ccsp_ops_linear_workspace(int32_t product, int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const void* a, int64_t a_stride, const void* b, int64_t b_stride) {
+    static const int32_t some = 0;
+    if (product < CCSP_OPS_FORWARD || product > CCSP_OPS_BACK_WEIGHT || check_linear("linear_workspace", type, n_experts, n_rows, inp, out, &some)) return -1;
+    int64_t bytes = 0;
+    dispatch_type(type, [&](auto t) { bytes = product_workspace<decltype(t)>(product, n_experts, n_rows, inp, out, a, a_stride, b, b_stride); return 0; });
+    return bytes;
+}
+
 int ccsp_ops_linear(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* x, int64_t x_stride, const void* weight, const void* bias,
-                    int32_t activation, void* y, void* z, void* stream) {
+                    int32_t activation, void* y, void* z, void* workspace, int64_t workspace_bytes, void* stream) {
     if (check_linear("linear", type, n_experts, n_rows, inp, out, offsets)) return 1;
     CCSP_OPS_CHECK(activation == CCSP_OPS_NONE || activation == CCSP_OPS_SILU, "linear: activation %d", activation);
     if (n_rows == 0) return 0;
     CCSP_OPS_CHECK(x && weight && y, "linear: null argument");
     ProdArgs p = {};
-    p.a = x; p.lda = x_stride; p.b = weight; p.ldb = inp; p.b_expert = inp * out; p.bias = bias; p.c = y; p.ldc = out; p.z = z;
-    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.seg_log2 = 31; p.N = (int)out; p.K = (int)inp; p.silu = activation == CCSP_OPS_SILU;
-    return dispatch_type(type, [&](auto t) { return launch_prod<decltype(t), PROD_FORWARD>(p, (hipStream_t)stream); });
+    p.bias = bias; p.c = y; p.ldc = out; p.z = z; p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.N = (int)out; p.K = (int)inp; p.silu = activation == CCSP_OPS_SILU;
+    p.seg_log2 = 31;
+    return dispatch_type(type, [&](auto t) { return run_product<decltype(t), PROD_FORWARD>(p, inp, out, x, x_stride, weight, inp, workspace, workspace_bytes, (hipStream_t)stream); });
 }
 
 int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, int64_t out, const int32_t* offsets, const void* dy, int64_t dy_stride, const void* z, void* dz, void* stream) {
@@ -107,44 +113,27 @@ int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, i
 }
 
 int ccsp_ops_linear_back_input(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride, const void* weight, void* dx,
-                               void* stream) {
+                               void* workspace, int64_t workspace_bytes, void* stream) {
     if (check_linear("linear_back_input", type, n_experts, n_rows, inp, out, offsets)) return 1;
     if (n_rows == 0) return 0;
     CCSP_OPS_CHECK(dz && weight && dx, "linear_back_input: null argument");
     ProdArgs p = {};
-    p.a = dz; p.lda = dz_stride; p.b = weight; p.ldb = inp; p.b_expert = inp * out; p.c = dx; p.ldc = inp;
-    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.seg_log2 = 31; p.N = (int)inp; p.K = (int)out;
-    return dispatch_type(type, [&](auto t) { return launch_prod<decltype(t), PROD_INPUT>(p, (hipStream_t)stream); });
-}
-
-int64_t ccsp_ops_linear_back_weight_workspace(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out) {
-    if (!type_ok(type) || n_experts < 1 || n_experts > CCSP_OPS_MAX_EXPERTS || n_rows < 0 || n_rows > CCSP_OPS_MAX_ASSIGN || inp < 1 || inp > CCSP_OPS_MAX_WIDTH || out < 1 || out > CCSP_OPS_MAX_WIDTH) return -1;
-    int64_t slots = 0;
-    dispatch_type(type, [&](auto t) {
-        const int l = seg_log2_for<decltype(t)>(n_rows, n_experts, out, inp);
-        slots = l == 31 ? 0 : 2 * ((n_rows >> l) + 1);
-        return 0;
-    });
-    return slots * (out * inp + out) * 4;
+    p.c = dx; p.ldc = inp; p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = -1; p.N = (int)inp; p.K = (int)out; p.seg_log2 = 31;
+    return dispatch_type(type, [&](auto t) { return run_product<decltype(t), PROD_INPUT>(p, inp, out, dz, dz_stride, weight, inp, workspace, workspace_bytes, (hipStream_t)stream); });
 }
 
 int ccsp_ops_linear_back_weight(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride, const void* x, int64_t x_stride,
                                 void* d_weight, void* d_bias, void* workspace, int64_t workspace_bytes, void* stream) {
     if (check_linear("linear_back_weight", type, n_experts, n_rows, inp, out, offsets)) return 1;
     CCSP_OPS_CHECK((n_rows == 0 || (dz && x)) && (d_weight || d_bias), "linear_back_weight: null argument");
-    const int64_t need = ccsp_ops_linear_back_weight_workspace(type, n_experts, n_rows, inp, out);
-    CCSP_OPS_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "linear_back_weight: workspace of %lld bytes is too small or not aligned to 16 bytes",
-                   (long long)workspace_bytes);
     ProdArgs p = {};
-    p.a = dz; p.lda = dz_stride; p.b = x; p.ldb = x_stride; p.c = d_weight; p.ldc = inp; p.c_expert = inp * out;
-    p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = (int)out; p.N = (int)inp; p.K = -1;
+    p.c = d_weight; p.ldc = inp; p.c_expert = inp * out; p.offsets = offsets; p.E = n_experts; p.R = (int)n_rows; p.M = (int)out; p.K = -1;
     p.sum = d_bias;                                              // (one kernel makes both; for the bias alone it goes over the first columns of x and writes no product)
-    p.parts = static_cast<float*>(workspace);
+    p.N = (int)(d_weight || inp < 64 ? inp : 64);
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;
-        p.seg_log2 = prod_direct<T, PROD_WEIGHT>(p) ? seg_log2_for<T>(n_rows, n_experts, out, inp) : 31;
-        if (!d_weight) p.N = p.N < 64 ? p.N : 64;
-        return launch_prod<T, PROD_WEIGHT>(p, (hipStream_t)stream);
+        p.seg_log2 = seg_log2_for<T>(n_rows, n_experts, out, inp);
+        return run_product<T, PROD_WEIGHT>(p, inp, out, dz, dz_stride, x, x_stride, workspace, workspace_bytes, (hipStream_t)stream);
     });
 }
 

@@ -20,6 +20,7 @@ struct ProdArgs {
     const int* offsets;
     int E, R, M, N, K;                                           // M, N, K of one expert's product; the one that is a row count is -1
     int silu;
+    int quads;                                                   // rows of the result take four elements at once: their number, stride and addresses are multiples
     float* parts;                                                // weight gradient of experts with more than 2^seg_log2 rows: [slot][M N + M] partial sums
     int seg_log2;                                                // 31: no expert's rows are cut
 };
@@ -65,155 +66,9 @@ template <typename T> struct Vec8 { typedef T t __attribute__((ext_vector_type(8
 __device__ __forceinline__ f32x4 mfma16(Vec8<bf16>::t a, Vec8<bf16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma16(Vec8<fp16>::t a, Vec8<fp16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// 16 bytes of a row of the operand along its contiguous side, `left` elements of it in range
-template <typename T>
-__device__ __forceinline__ u32x4 load_piece(const T* p, int left) {
-    constexpr int V = 16 / sizeof(T);
-    union { T e[V]; u32x4 v; } x;
-    x.v = u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < V; ++i) if (i < left) x.e[i] = p[i];
-    return x.v;
-}
-
 // ------------------------------------------------------------------------------------------------------------------------
-// 16-bit types, rows of any alignment.  Tile 128 x 128 x 64, 4 waves as 2 x 2, each 64 x 64 as 4 x 4 tiles of v_mfma 16x16x32; the operands are handed over in exchanged roles
-// (n on the rows of the result), so that a lane holds four consecutive n of one m and stores them as one access.
-// LDS holds an operand in pieces of 16 bytes.  k contiguous: [128 rows][8 pieces], piece c of row r at c ^ (r & 7): the 16 lanes of a fragment
-// read touch every bank alike.  k across rows: [64 k][128], read by ds_read_tr16_b64, which hands lane i of 16 the column i of a 4 x 16 block; the
-// block's 32 bytes sit at (column / 16) ^ (k & 3 | (k >> 3 & 1) << 2), so that the 16 row segments of an access spread over the banks.
-// ------------------------------------------------------------------------------------------------------------------------
-constexpr int PT = 128, PK = 64;
-
-template <bool KC> __device__ __forceinline__ int lds_piece(int row, int c) {      // element index of piece c of row `row` (KC: row = m or n; else row = k)
-    if (KC) return row * PK + ((c ^ (row & 7)) << 3);
-    const int f = (row & 3) | ((row >> 3 & 1) << 2);
-    return row * PT + ((((c >> 1) ^ f) << 1 | (c & 1)) << 3);
-}
-
-template <typename T, bool KC>
-__device__ __forceinline__ typename Vec8<T>::t lds_frag(const T* s, int r0, int ks) {
-    typedef typename Vec8<T>::t V8;
-    const int lane = threadIdx.x & 63, q = lane >> 4, i = lane & 15;
-    if constexpr (KC) {
-        return *reinterpret_cast<const V8*>(s + lds_piece<true>(r0 + i, ks * 4 + q));
-    } else {
-        typedef __attribute__((address_space(3))) s16x4* P;
-        union { s16x4 h[2]; V8 v; } x;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = 32 * ks + 8 * q + 4 * h + (i >> 2), f = (k & 3) | ((k >> 3 & 1) << 2);
-            x.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(s + k * PT + (((r0 >> 4) ^ f) << 4) + 4 * (i & 3)));
-        }
-        return x.v;
-    }
-}
-
-template <typename T, int PROD>
-__global__ __launch_bounds__(256) void k_prod16(ProdArgs p, int tiles_n) {
-    constexpr bool AKC = PROD != PROD_WEIGHT, BKC = PROD == PROD_FORWARD;
-    __shared__ __attribute__((aligned(16))) T sA[PT * PK], sB[PT * PK];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    const int bid = blockIdx.x;
-    int e, r0 = 0, r1 = 0, m0, n0, M, K;
-    if (PROD == PROD_WEIGHT) {
-        const int tiles_m = (p.M + PT - 1) / PT;
-        e = bid / (tiles_m * tiles_n);
-        const int t = bid - e * tiles_m * tiles_n;
-        m0 = t / tiles_n * PT; n0 = t % tiles_n * PT; M = p.M;
-        r0 = p.offsets[e]; K = p.offsets[e + 1] - r0;
-    } else {
-        if (!find_tile(p.offsets, p.E, p.R, 7, bid / tiles_n, &e, &r0, &r1)) return;
-        m0 = 0; n0 = bid % tiles_n * PT; M = r1 - r0 < PT ? r1 - r0 : PT; K = e < p.E ? p.K : 0;
-    }
-    const int N = p.N;
-    const T* A = static_cast<const T*>(p.a) + (PROD == PROD_WEIGHT ? (long)r0 * p.lda + m0 : (long)r0 * p.lda);
-    const T* B = static_cast<const T*>(p.b) + (PROD == PROD_WEIGHT ? (long)r0 * p.ldb + n0 : e * p.b_expert + (BKC ? (long)n0 * p.ldb : (long)n0));
-    const int left_m = M - m0, left_n = N - n0;
-    u32x4 ra[4], rb[4];
-    auto load = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int x = tid + 256 * i;
-            if (AKC) { const int r = x >> 3, c = x & 7; ra[i] = load_piece<T>(A + (long)r * p.lda + k0 + 8 * c, r < left_m ? K - k0 - 8 * c : 0); }
-            else { const int k = x >> 4, c = x & 15; ra[i] = load_piece<T>(A + (long)(k0 + k) * p.lda + 8 * c, k0 + k < K ? left_m - 8 * c : 0); }
-            if (BKC) { const int r = x >> 3, c = x & 7; rb[i] = load_piece<T>(B + (long)r * p.ldb + k0 + 8 * c, r < left_n ? K - k0 - 8 * c : 0); }
-            else { const int k = x >> 4, c = x & 15; rb[i] = load_piece<T>(B + (long)(k0 + k) * p.ldb + 8 * c, k0 + k < K ? left_n - 8 * c : 0); }
-        }
-    };
-    f32x4 acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const bool sums = PROD == PROD_WEIGHT && p.sum && n0 + wn == 0;
-    f32x4 sum[4] = {};
-    typename Vec8<T>::t ones;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = (T)1.0f;
-    if (K > 0) load(0);
-    for (int k0 = 0; k0 < K; k0 += PK) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int x = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(sA + (AKC ? lds_piece<true>(x >> 3, x & 7) : lds_piece<false>(x >> 4, x & 15))) = ra[i];
-            *reinterpret_cast<u32x4*>(sB + (BKC ? lds_piece<true>(x >> 3, x & 7) : lds_piece<false>(x >> 4, x & 15))) = rb[i];
-        }
-        __syncthreads();
-        if (k0 + PK < K) load(k0 + PK);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            typename Vec8<T>::t fa[4], fb[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { fa[i] = lds_frag<T, AKC>(sA, wm + 16 * i, ks); fb[i] = lds_frag<T, BKC>(sB, wn + 16 * i, ks); }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = mfma16(fb[j], fa[i], acc[i][j]);
-            if (sums) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] = mfma16(ones, fa[i], sum[i]);
-            }
-        }
-    }
-    T* C = static_cast<T*>(p.c) + (PROD == PROD_WEIGHT ? e * p.c_expert + (long)m0 * p.ldc : (long)r0 * p.ldc);
-    T* Z = PROD == PROD_FORWARD && p.z ? static_cast<T*>(p.z) + (long)r0 * p.ldc : nullptr;
-    const T* bias = PROD == PROD_FORWARD && p.bias && e < p.E ? static_cast<const T*>(p.bias) + (long)e * N : nullptr;
-    const bool silu = PROD == PROD_FORWARD && p.silu && e < p.E;
-    if (sums && lane < 16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (wm + 16 * i + lane < left_m) static_cast<T*>(p.sum)[(long)e * p.M + m0 + wm + 16 * i + lane] = (T)sum[i][0];
-    }
-    if (PROD == PROD_WEIGHT && !p.c) return;                     // (the sums alone)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
-        float bv[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) bv[r] = bias && n + r < N ? (float)bias[n + r] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int m = wm + 16 * i + (lane & 15);
-            if (m >= left_m || n >= N) continue;
-            typename VecOf<T, 4>::type y, z;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float v = acc[i][j][r] + bv[r];
-                z[r] = (T)v;
-                y[r] = silu ? (T)silu_value(v) : (T)v;
-            }
-            const long at = (long)m * p.ldc + n;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (n + r < N) { C[at + r] = y[r]; if (Z) Z[at + r] = z[r]; }
-        }
-    }
-}
-
-// ------------------------------------------------------------------------------------------------------------------------
-// 16-byte rows: the operands go from memory to LDS without passing a register (buffer_load ... lds), a stage ahead of the products.
+// The operands go from memory to LDS without passing a register (buffer_load ... lds), NST - 1 stages ahead of the products.  Their rows are whole 16-byte
+// pieces at multiples of 16 bytes; rows that are not are copied and padded first (k_pad_rows).
 // A lane's 16 bytes land at a fixed place of its wave's 1 KB, so the swizzle of a layout is made by choosing which bytes a lane asks for; what is out
 // of range (rows past the group, columns past the matrix, k past its end) is asked for past the buffer's end and arrives as zeros.  The buffer's base
 // advances with k, so that no offset inside it passes 31 bits however long a group is.
@@ -225,7 +80,7 @@ __global__ __launch_bounds__(256) void k_prod16(ProdArgs p, int tiles_n) {
 // 32 bits use v_mfma_f32_32x32x2_f32 (products and sums in 32 bits throughout); its two k are taken 4 apart, so that a lane's k of four instructions are
 // one 16-byte read where k is contiguous.
 //
-// TM x TN by WM x WN waves, two LDS stages.  A wave's TM / WM x TN / WN part decides how many LDS bytes a product costs: in 16 bits the LDS port is as
+// TM x TN by WM x WN waves.  A wave's TM / WM x TN / WN part decides how many LDS bytes a product costs: in 16 bits the LDS port is as
 // busy as the matrix pipe at 64 x 64 and three quarters of it at 128 x 64.
 // ------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void lds_dma16(u32x4 rsrc, unsigned int offset, unsigned int lds) {
@@ -233,11 +88,12 @@ __device__ __forceinline__ void lds_dma16(u32x4 rsrc, unsigned int offset, unsig
 }
 constexpr unsigned int DMA_OUT = 0x80000000u;                    // an offset past every buffer
 
+// 16 bits, k across rows: which 32-byte block a block of k row k goes to (R / 16 blocks a row)
+template <int R> __device__ __forceinline__ int block_swizzle(int k) { return ((k & 3) | ((k >> 3 & 1) << 2)) & (R / 16 - 1); }
 // place of piece c in k row k (k across rows)
-template <typename T> __device__ __forceinline__ int across_piece(int k, int c) {
+template <typename T, int R> __device__ __forceinline__ int across_piece(int k, int c) {
     if (sizeof(T) == 4) return c ^ (k >> 2 & 1) << 3;
-    const int f = (k & 3) | ((k >> 3 & 1) << 2);
-    return ((c >> 1) ^ f) << 1 | (c & 1);
+    return ((c >> 1) ^ block_swizzle<R>(k)) << 1 | (c & 1);
 }
 
 // one operand of a block: R rows (m or n) by K, staged 128 bytes of k at a time
@@ -264,7 +120,7 @@ struct Stager {
                 off[i] = r < left ? (unsigned int)(r * row_bytes + c * 16) : DMA_OUT;
             } else {
                 constexpr int CH = R / V;                        // pieces of 16 bytes in a k row
-                const int x = at * 64 + lane, k = x / CH, c = across_piece<T>(k, x % CH);      // (the swizzle is its own inverse)
+                const int x = at * 64 + lane, k = x / CH, c = across_piece<T, R>(k, x % CH);      // (the swizzle is its own inverse)
                 off[i] = V * c < left ? (unsigned int)(k * row_bytes + c * 16) : DMA_OUT;
             }
         }
@@ -294,14 +150,15 @@ __device__ __forceinline__ typename Vec8<T>::t stage_frag(const T* s, int r0, in
     typedef typename Vec8<T>::t V8;
     const int lane = threadIdx.x & 63, q = lane >> 4, i = lane & 15;
     if constexpr (KC) {
-        return *reinterpret_cast<const V8*>(s + lds_piece<true>(r0 + i, ks * 4 + q));
+        const int r = r0 + i;
+        return *reinterpret_cast<const V8*>(s + r * 64 + (((ks * 4 + q) ^ (r & 7)) << 3));
     } else {
         typedef __attribute__((address_space(3))) s16x4* P;
         union { s16x4 h[2]; V8 v; } x;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int k = 32 * ks + 8 * q + 4 * h + (i >> 2), f = (k & 3) | ((k >> 3 & 1) << 2);
-            x.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(s + k * R + (((r0 >> 4) ^ f) << 4) + 4 * (i & 3)));
+            const int k = 32 * ks + 8 * q + 4 * h + (i >> 2);
+            x.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(s + k * R + (((r0 >> 4) ^ block_swizzle<R>(k)) << 4) + 4 * (i & 3)));
         }
         return x.v;
     }
@@ -334,12 +191,14 @@ __device__ __forceinline__ void tile_order(int b, int tiles_m, int tiles_n, int*
 // starts are more than 2^l apart, so first segments differ in first >> l; segment i > 0 has (first >> l) + i, which is at most (end >> l), and the
 // next expert's second segment at least one more.)
 __host__ __device__ __forceinline__ int seg_slot(int first, int i, int l) { return 2 * ((first >> l) + i) + (i > 0); }
+// a slot: the product, the sums, rounded up to 16 bytes
+__host__ __device__ __forceinline__ long part_floats(long M, long N) { return (M * N + M + 3) & ~3l; }
 
 template <int V> struct Log2 { static constexpr int v = 1 + Log2<V / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
-template <typename T, int PROD, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_prod_direct(ProdArgs p, int tiles_m, int tiles_n) {
+template <typename T, int PROD, int TM, int TN, int WM, int WN, int NST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int tiles_m, int tiles_n) {
     constexpr bool AKC = PROD != PROD_WEIGHT, BKC = PROD == PROD_FORWARD, F32 = sizeof(T) == 4;
     constexpr int G = F32 ? 32 : 16, FA = TM / WM / G, FB = TN / WN / G, RG = F32 ? 16 : 4;      // fragment side, fragments, result registers
     constexpr int SK = 128 / sizeof(T), STAGE = (TM + TN) * SK;
@@ -357,7 +216,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod_direct(ProdArgs p, int
             if (!find_tile(p.offsets, p.E, p.offsets[p.E], p.seg_log2, t, &e, &r0, &r1)) return;
             const int first = p.offsets[e], i = (r0 - first) >> p.seg_log2;
             K = r1 - r0 < 1 << p.seg_log2 ? r1 - r0 : 1 << p.seg_log2;
-            if (r1 - first > 1 << p.seg_log2) part = p.parts + (long)seg_slot(first, i, p.seg_log2) * ((long)p.M * p.N + p.M);
+            if (r1 - first > 1 << p.seg_log2) part = p.parts + seg_slot(first, i, p.seg_log2) * part_floats(p.M, p.N);
         }
         m0 = tm * TM;
         M = p.M;
@@ -383,18 +242,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod_direct(ProdArgs p, int
         ga.init(A, p.lda, left_m);
         gb.init(B, p.ldb, N - n0);
         const unsigned int l0 = (unsigned int)(unsigned long)(__attribute__((address_space(3))) unsigned short*)lds;
-        ga.load(l0, K);
-        gb.load(l0 + TM * 128, K);
+        constexpr int BYTES = STAGE * (int)sizeof(T), LOADS = (NST - 2) * (ga.N + gb.N);        // of a stage; of the stages that may be on their way
+        static_assert(LOADS < 64, "the wait's counter");
+#pragma unroll
+        for (int i = 0; i < NST - 1; ++i)
+            if (i * SK < K) { ga.load(l0 + i * BYTES, K - i * SK); gb.load(l0 + i * BYTES + TM * 128, K - i * SK); }
         auto loop = [&](auto with_sums) {
             constexpr bool S = decltype(with_sums)::value;
             int buf = 0;
-            for (int k0 = 0; k0 < K; k0 += SK, buf ^= 1) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wave's part of the stage is there;
-                __syncthreads();                                 // everyone's, and nobody reads the other stage any more
-                if (k0 + SK < K) {
-                    const unsigned int l1 = l0 + (buf ^ 1) * STAGE * (int)sizeof(T);
-                    ga.load(l1, K - k0 - SK);
-                    gb.load(l1 + TM * 128, K - k0 - SK);
+            for (int k0 = 0; k0 < K; k0 += SK, buf = buf + 1 == NST ? 0 : buf + 1) {
+                // this wave's part of the stage is there (its loads come back in order, NST - 2 later stages may be on their way);
+                if (k0 + (NST - 2) * SK < K) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();                    // everyone's, and nobody reads the stage before it any more (its reads have come back)
+                asm volatile("" ::: "memory");
+                if (k0 + (NST - 1) * SK < K) {
+                    const unsigned int l1 = l0 + (buf == 0 ? NST - 1 : buf - 1) * BYTES;
+                    ga.load(l1, K - k0 - (NST - 1) * SK);
+                    gb.load(l1 + TM * 128, K - k0 - (NST - 1) * SK);
                 }
                 const T *sA = sm + buf * STAGE, *sB = sA + TM * SK;
                 if constexpr (F32) {
@@ -457,18 +322,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod_direct(ProdArgs p, int
 #pragma unroll
         for (int g = 0; g < RG / 4; ++g) {
             const int n = n0 + wn + G * j + (F32 ? 8 * g + 4 * (lane >> 5) : 4 * (lane >> 4));
-            if (n >= N) continue;                                // (N is a multiple of 4: four columns are in or out together)
+            if (n >= N) continue;
+            const int left_n = N - n < 4 ? N - n : 4;
             float bv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (bias) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) bv[r] = (float)bias[n + r];
+                for (int r = 0; r < 4; ++r) bv[r] = r < left_n ? (float)bias[n + r] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < FA; ++i) {
                 const int m = wm + G * i + (lane & (G - 1));
                 if (m >= left_m) continue;
                 if (PROD == PROD_WEIGHT && part) {
-                    *reinterpret_cast<f32x4*>(part + (long)(m0 + m) * N + n) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                    float* const to = part + (long)(m0 + m) * N + n;
+                    if (p.quads) *reinterpret_cast<f32x4*>(to) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                    else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) if (r < left_n) to[r] = acc[i][j][4 * g + r];
+                    }
                     continue;
                 }
                 V4 y, z;
@@ -478,150 +349,61 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_prod_direct(ProdArgs p, int
                     z[r] = (T)v;
                     y[r] = silu ? (T)silu_value(v) : (T)v;
                 }
-                *reinterpret_cast<V4*>(C + (long)m * p.ldc + n) = y;
-                if (Z) *reinterpret_cast<V4*>(Z + (long)m * p.ldc + n) = z;
-            }
-        }
-}
-
-// ------------------------------------------------------------------------------------------------------------------------
-// 32 bits, rows of any alignment.  Tile 64 x 64 x 32, 4 waves as 2 x 2.  LDS: k contiguous [64][33], else [32][68]: one word per lane and fragment, no two lanes on one bank.
-// ------------------------------------------------------------------------------------------------------------------------
-constexpr int TS = 64, FK = 32, FLD_KC = FK + 1;
-template <bool KC> __device__ __forceinline__ int f32_at(int r, int k) { return KC ? r * FLD_KC + k : k * (TS + 4) + r; }
-
-template <int PROD>
-__global__ __launch_bounds__(256) void k_prod32(ProdArgs p, int tiles_n) {
-    constexpr bool AKC = PROD != PROD_WEIGHT, BKC = PROD == PROD_FORWARD;
-    __shared__ __attribute__((aligned(16))) float sA[FK * (TS + 4)], sB[FK * (TS + 4)];
-    constexpr int F = TS / 64, NP = TS / 32, CH = TS / 4;          // fragments of a wave's side, pieces of a thread, pieces of a k row
-    static_assert(TS * FLD_KC <= FK * (TS + 4), "both layouts fit");
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * (TS / 2), wn = (wave & 1) * (TS / 2);
-    const int bid = blockIdx.x;
-    int e, r0 = 0, r1 = 0, m0, n0, M, K;
-    if (PROD == PROD_WEIGHT) {
-        const int tiles_m = (p.M + TS - 1) / TS;
-        e = bid / (tiles_m * tiles_n);
-        const int t = bid - e * tiles_m * tiles_n;
-        m0 = t / tiles_n * TS; n0 = t % tiles_n * TS; M = p.M;
-        r0 = p.offsets[e]; K = p.offsets[e + 1] - r0;
-    } else {
-        if (!find_tile(p.offsets, p.E, p.R, 6, bid / tiles_n, &e, &r0, &r1)) return;
-        m0 = 0; n0 = bid % tiles_n * TS; M = r1 - r0 < TS ? r1 - r0 : TS; K = e < p.E ? p.K : 0;
-    }
-    const int N = p.N;
-    const float* A = static_cast<const float*>(p.a) + (PROD == PROD_WEIGHT ? (long)r0 * p.lda + m0 : (long)r0 * p.lda);
-    const float* B = static_cast<const float*>(p.b) + (PROD == PROD_WEIGHT ? (long)r0 * p.ldb + n0 : e * p.b_expert + (BKC ? (long)n0 * p.ldb : (long)n0));
-    const int left_m = M - m0, left_n = N - n0;
-    u32x4 ra[NP], rb[NP];
-    auto load = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int x = tid + 256 * i;
-            if (AKC) { const int r = x >> 3, c = x & 7; ra[i] = load_piece<float>(A + (long)r * p.lda + k0 + 4 * c, r < left_m ? K - k0 - 4 * c : 0); }
-            else { const int k = x / CH, c = x % CH; ra[i] = load_piece<float>(A + (long)(k0 + k) * p.lda + 4 * c, k0 + k < K ? left_m - 4 * c : 0); }
-            if (BKC) { const int r = x >> 3, c = x & 7; rb[i] = load_piece<float>(B + (long)r * p.ldb + k0 + 4 * c, r < left_n ? K - k0 - 4 * c : 0); }
-            else { const int k = x / CH, c = x % CH; rb[i] = load_piece<float>(B + (long)(k0 + k) * p.ldb + 4 * c, k0 + k < K ? left_n - 4 * c : 0); }
-        }
-    };
-    auto put = [&](float* s, bool kc, int x, u32x4 v) {
-        if (kc) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[(x >> 3) * FLD_KC + 4 * (x & 7) + j] = __uint_as_float(v[j]);
-        } else *reinterpret_cast<u32x4*>(s + x / CH * (TS + 4) + 4 * (x % CH)) = v;
-    };
-    f32x16 acc[F][F], sum[F];
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            sum[i][r] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < F; ++j) acc[i][j][r] = 0.0f;
-        }
-    const bool sums = PROD == PROD_WEIGHT && p.sum && n0 + wn == 0;
-    if (K > 0) load(0);
-    for (int k0 = 0; k0 < K; k0 += FK) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NP; ++i) { put(sA, AKC, tid + 256 * i, ra[i]); put(sB, BKC, tid + 256 * i, rb[i]); }
-        __syncthreads();
-        if (k0 + FK < K) load(k0 + FK);
-#pragma unroll
-        for (int k = 0; k < FK; k += 2) {
-            float fa[F], fb[F];
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                fa[i] = sA[f32_at<AKC>(wm + 32 * i + (lane & 31), k + (lane >> 5))];
-                fb[i] = sB[f32_at<BKC>(wn + 32 * i + (lane & 31), k + (lane >> 5))];
-            }
-#pragma unroll
-            for (int i = 0; i < F; ++i)
-#pragma unroll
-                for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j], fa[i], acc[i][j], 0, 0, 0);
-            if (sums) {
-#pragma unroll
-                for (int i = 0; i < F; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(1.0f, fa[i], sum[i], 0, 0, 0);
-            }
-        }
-    }
-    float* C = static_cast<float*>(p.c) + (PROD == PROD_WEIGHT ? e * p.c_expert + (long)m0 * p.ldc : (long)r0 * p.ldc);
-    float* Z = PROD == PROD_FORWARD && p.z ? static_cast<float*>(p.z) + (long)r0 * p.ldc : nullptr;
-    const float* bias = PROD == PROD_FORWARD && p.bias && e < p.E ? static_cast<const float*>(p.bias) + (long)e * N : nullptr;
-    const bool silu = PROD == PROD_FORWARD && p.silu && e < p.E;
-    if (sums && lane < 32) {
-#pragma unroll
-        for (int i = 0; i < F; ++i)
-            if (wm + 32 * i + lane < left_m) static_cast<float*>(p.sum)[(long)e * p.M + m0 + wm + 32 * i + lane] = sum[i][0];
-    }
-    if (PROD == PROD_WEIGHT && !p.c) return;                     // (the sums alone)
-#pragma unroll
-    for (int j = 0; j < F; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int n = n0 + wn + 32 * j + 8 * g + 4 * (lane >> 5);
-            float bv[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bv[r] = bias && n + r < N ? bias[n + r] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                const int m = wm + 32 * i + (lane & 31);
-                if (m >= left_m || n >= N) continue;
-                f32x4 y, z;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) { z[r] = acc[i][j][4 * g + r] + bv[r]; y[r] = silu ? silu_value(z[r]) : z[r]; }
                 const long at = (long)m * p.ldc + n;
+                if (p.quads) {
+                    *reinterpret_cast<V4*>(C + at) = y;
+                    if (Z) *reinterpret_cast<V4*>(Z + at) = z;
+                } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < N) { C[at + r] = y[r]; if (Z) Z[at + r] = z[r]; }
+                    for (int r = 0; r < 4; ++r)
+                        if (r < left_n) { C[at + r] = y[r]; if (Z) Z[at + r] = z[r]; }
+                }
             }
         }
 }
 
 // The weight gradient of experts whose rows were cut, their segments' partial sums added in order; zeros for experts without rows (they have no
-// segment); the rest is there already.  x: 1024 values of M N and M, y: expert
-template <typename T>
+// segment); the rest is there already.  V values (of M N, then of M) a thread, y: expert
+template <typename T, int V>
 __global__ __launch_bounds__(256) void k_join_parts(ProdArgs p) {
     const int e = blockIdx.y, first = p.offsets[e], n = p.offsets[e + 1] - first, l = p.seg_log2;
     if (n > 0 && n <= 1 << l) return;
-    const long mn = (long)p.M * p.N, all = mn + (p.sum ? p.M : 0);
+    const long mn = (long)p.M * p.N, all = mn + (p.sum ? p.M : 0), slot = part_floats(p.M, p.N);
     const int segs = (n + (1 << l) - 1) >> l;
-    typedef typename VecOf<T, 4>::type V4;
-    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (long)gridDim.x * 1024) {       // (M N and M are multiples of 4)
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    typedef typename VecOf<T, V>::type VT;
+    typedef typename VecOf<float, V>::type VF;
+    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * V; i < all; i += (long)gridDim.x * 256 * V) {
+        float v[V] = {};
         for (int k = 0; k < segs; ++k) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(p.parts + (long)seg_slot(first, k, l) * (mn + p.M) + i);
+            const VF a = *reinterpret_cast<const VF*>(p.parts + seg_slot(first, k, l) * slot + i);
+            const float* ae = reinterpret_cast<const float*>(&a);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += a[r];
+            for (int r = 0; r < V; ++r) v[r] += ae[r];
         }
-        V4 o;
+        VT o;
+        T* oe = reinterpret_cast<T*>(&o);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
-        if (i < mn) { if (p.c) *reinterpret_cast<V4*>(static_cast<T*>(p.c) + e * p.c_expert + i) = o; }
+        for (int r = 0; r < V; ++r) oe[r] = (T)v[r];
+        if (i < mn) { if (p.c) *reinterpret_cast<VT*>(static_cast<T*>(p.c) + e * p.c_expert + i) = o; }
         else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) static_cast<T*>(p.sum)[(long)e * p.M + i - mn + r] = o[r];
+            for (int r = 0; r < V; ++r) static_cast<T*>(p.sum)[(long)e * p.M + i - mn + r] = oe[r];
         }
+    }
+}
+
+// rows of any width, stride and address as rows of whole 16-byte pieces, zeros behind the width
+template <typename T>
+__global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ src, long rows, int width, long stride, T* __restrict__ dst, int pieces) {
+    constexpr int V = 16 / sizeof(T);
+    const long n = rows * pieces;
+    for (long i = block_id() * 256 + threadIdx.x; i < n; i += (long)gridDim.x * gridDim.y * 256) {
+        const long r = i / pieces;
+        const int c = (int)(i - r * pieces) * V;
+        union { T e[V]; u32x4 v; } x;
+#pragma unroll
+        for (int j = 0; j < V; ++j) x.e[j] = c + j < width ? src[r * stride + c + j] : (T)0.0f;
+        *reinterpret_cast<u32x4*>(dst + i * V) = x.v;
     }
 }
 
@@ -643,65 +425,122 @@ __global__ __launch_bounds__(256) void k_silu_back(const int* __restrict__ activ
     }
 }
 
-template <typename T, int PROD, int TM, int TN, int WM, int WN>
-int launch_direct(const ProdArgs& p, hipStream_t s) {
+template <typename T, int PROD, int TM, int TN, int WM, int WN, int NST>
+int launch_tiles(const ProdArgs& p, hipStream_t s) {
     const long tn = cdiv(p.N, TN), tm = PROD == PROD_WEIGHT ? cdiv(p.M, TM) : most_tiles(p.R, p.E, Log2<TM>::v);
     const bool cut = PROD == PROD_WEIGHT && p.seg_log2 != 31;
     const long blocks = (PROD == PROD_WEIGHT ? (cut ? most_tiles(p.R, p.E, p.seg_log2) : p.E) : 1) * tm * tn;
     if (blocks > 0x003fffffL) return fail("expert_linear: %ld tiles are more than a launch holds", blocks);
-    if (blocks) hipLaunchKernelGGL((k_prod_direct<T, PROD, TM, TN, WM, WN>), dim3((unsigned)blocks), dim3(64 * WM * WN), 2 * (TM + TN) * 128, s, p, (int)tm, (int)tn);
+    if (blocks) hipLaunchKernelGGL((k_product<T, PROD, TM, TN, WM, WN, NST>), dim3((unsigned)blocks), dim3(64 * WM * WN), NST * (TM + TN) * 128, s, p, (int)tm, (int)tn);
     if (cut) {
-        const long per = cdiv((long)p.M * p.N + p.M, 1024);
-        hipLaunchKernelGGL(k_join_parts<T>, dim3((unsigned)(per < 1024 ? per : 1024), p.E), dim3(256), 0, s, p);
+        const bool four = p.quads && p.M % 4 == 0;
+        const long per = cdiv((long)p.M * p.N + p.M, four ? 1024 : 256);
+        const dim3 grid((unsigned)(per < 1024 ? per : 1024), p.E);
+        if (four) hipLaunchKernelGGL((k_join_parts<T, 4>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((k_join_parts<T, 1>), grid, dim3(256), 0, s, p);
     }
     LAUNCHED();
     return 0;
 }
 
-template <typename K>
-int launch_any(K kernel, const ProdArgs& p, bool weight, int ts_log2, hipStream_t s) {
-    const long tn = cdiv(p.N, 1 << ts_log2), blocks = weight ? (long)p.E * cdiv(p.M, 1 << ts_log2) * tn : most_tiles(p.R, p.E, ts_log2) * tn;
-    if (blocks > 0x00ffffffL) return fail("expert_linear: %ld tiles are more than a launch holds", blocks);
-    if (blocks == 0) return 0;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, s, p, (int)tn);
-    LAUNCHED();
-    return 0;
-}
-
-// The tile of a product: 256 x 256 where there are enough of them to go round the CUs a few times (E: groups, for the weight gradient with tiles of its own)
+// Tiles of a product by how many there are: 256 x 256 where they go round the CUs a few times, 128 x 128, and 64 x 64 with four stages where even
+// those are too few to keep enough bytes on their way (one token's experts, short prompts).  A weight gradient over few rows an expert writes more than it
+// multiplies: there two blocks a CU write while another multiplies (32 experts of 256 rows, 2048 x 1408: 110 us by 128, 128 us by 256).
+inline long prod_tiles(bool weight, long R, long E, long M, long N, int l) { return (weight ? E * cdiv(M, 1l << l) : most_tiles(R, E, l)) * cdiv(N, 1l << l); }
+enum { TILE_64 = 6, TILE_128 = 7, TILE_256 = 8 };
 template <typename T>
-bool prod_big(bool weight, long R, long E, long M, long N) { return sizeof(T) == 2 && (weight ? E * cdiv(M, 256) : most_tiles(R, E, 8)) * cdiv(N, 256) >= 1024; }
+int prod_tile(bool weight, long R, long E, long M, long N) {
+    if (sizeof(T) == 4) return TILE_64;
+    if (prod_tiles(weight, R, E, M, N, 8) >= 1024 && (!weight || R >= 1024 * E)) return TILE_256;
+    return prod_tiles(weight, R, E, M, N, 7) >= 512 ? TILE_128 : TILE_64;
+}
 
 // Rows of a segment of the weight gradient (log2; 31: uncut).  An expert's tile is one block's chain over all of its rows, so a few long experts would
 // leave most CUs idle: rows are cut until there are about four blocks a CU.  A segment's partial sums cost 8 bytes a value to write and add, which
 // its products have to be worth.
 template <typename T>
 int seg_log2_for(long R, long E, long M, long N) {
-    if (prod_big<T>(true, R, E, M, N)) return 31;
-    constexpr int TS = sizeof(T) == 4 ? 64 : 128, least = sizeof(T) == 4 ? 9 : 10;
-    const long want = R * cdiv(M, TS) * cdiv(N, TS) / 1024;
+    const int tile = prod_tile<T>(true, R, E, M, N);
+    if (tile == TILE_256) return 31;
+    const int least = sizeof(T) == 4 ? 9 : 10;
+    const long want = R * cdiv(M, 1l << tile) * cdiv(N, 1l << tile) / 1024;
     int l = least;
     while (l < 30 && (2l << l) <= want) ++l;
     return (1l << l) >= R ? 31 : l;
 }
 
 template <typename T, int PROD>
-bool prod_direct(const ProdArgs& p) {
-    constexpr int V = 16 / sizeof(T);
-    // every address and stride a multiple of 16 bytes, no piece that is partly out, an offset inside a stage below 2^31
-    return common_align({(uint64_t)(uintptr_t)p.a, (uint64_t)(uintptr_t)p.b, (uint64_t)(uintptr_t)p.c, (uint64_t)(uintptr_t)p.z, (uint64_t)p.lda * sizeof(T), (uint64_t)p.ldb * sizeof(T),
-                         (uint64_t)p.ldc * sizeof(T)}) == 16 &&
-           p.N % V == 0 && (PROD == PROD_WEIGHT ? p.M % V == 0 : p.K % V == 0) && p.lda < (1 << 21) && p.ldb < (1 << 21);
-}
-
-template <typename T, int PROD>
 int launch_prod(const ProdArgs& p, hipStream_t s) {
     constexpr bool W = PROD == PROD_WEIGHT;
-    if constexpr (sizeof(T) == 4) {
-        if (prod_direct<T, PROD>(p)) return launch_direct<T, PROD, 64, 64, 2, 2>(p, s);
-        return launch_any(k_prod32<PROD>, p, W, 6, s);
+    const int tile = prod_tile<T>(W, p.R, p.E, p.M, p.N);
+    if constexpr (sizeof(T) == 2) {
+        if (tile == TILE_256) return launch_tiles<T, PROD, 256, 256, 2, 4, 2>(p, s);
+        if (tile == TILE_128) return launch_tiles<T, PROD, 128, 128, 2, 2, 2>(p, s);
+        return launch_tiles<T, PROD, 64, 64, 2, 2, 4>(p, s);
     } else {
-        if (prod_direct<T, PROD>(p)) return prod_big<T>(W, p.R, p.E, p.M, p.N) ? launch_direct<T, PROD, 256, 256, 2, 4>(p, s) : launch_direct<T, PROD, 128, 128, 2, 2>(p, s);
-        return launch_any(k_prod16<T, PROD>, p, W, 7, s);
+        return launch_tiles<T, PROD, 64, 64, 2, 2, 2>(p, s);
     }
+}
+
+// An operand as the products read it: in place, or copied into the workspace with rows of whole pieces.
+template <typename T>
+struct Operand {
+    const void* p; long rows, width, stride;
+    bool fits() const {                                          // (rows that lie on each other are copied too: a buffer's end is a number of rows)
+        constexpr long V = 16 / sizeof(T);
+        return ((uintptr_t)p & 15) == 0 && width % V == 0 && stride % V == 0 && stride >= width && stride < (1 << 21);
+    }
+    long padded() const { constexpr long V = 16 / sizeof(T); return (width + V - 1) / V * V; }
+    int64_t bytes() const { return fits() ? 0 : (rows * padded() * (long)sizeof(T) + 255) & ~255l; }
+    // in place of the operand: where it is and its stride; advances the workspace
+    void place(const void** at, long* ld, char** ws, hipStream_t s) const {
+        *at = p; *ld = stride;
+        if (fits()) return;
+        const int pieces = (int)(padded() * (long)sizeof(T) / 16);
+        const long blocks = cdiv(rows * pieces, 256);
+        if (blocks) hipLaunchKernelGGL(k_pad_rows<T>, grid_of(blocks < 16384 ? blocks : 16384), dim3(256), 0, s, (const T*)p, rows, (int)width, stride, (T*)*ws, pieces);
+        *at = *ws; *ld = padded();
+        *ws += bytes();
+    }
+};
+template <typename T>
+bool quads_ok(long N, long ldc, const void* c, const void* z) { return N % 4 == 0 && ldc % 4 == 0 && (((uintptr_t)c | (uintptr_t)z) & (4 * sizeof(T) - 1)) == 0; }
+
+// the operands of a product, as the entry points name them
+template <typename T>
+void linear_operands(int32_t product, int64_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const void* a, int64_t a_stride, const void* b, int64_t b_stride, Operand<T>* oa,
+                            Operand<T>* ob) {
+    *oa = {a, (long)n_rows, (long)(product == CCSP_OPS_FORWARD ? inp : out), (long)a_stride};
+    if (product == CCSP_OPS_BACK_WEIGHT) *ob = {b, (long)n_rows, (long)inp, (long)b_stride};
+    else *ob = {b, (long)(n_experts * out), (long)inp, (long)inp};
+}
+
+template <typename T>
+int64_t product_workspace(int32_t product, int64_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const void* a, int64_t a_stride, const void* b, int64_t b_stride) {
+    Operand<T> oa, ob;
+    linear_operands<T>(product, n_experts, n_rows, inp, out, a, a_stride, b, b_stride, &oa, &ob);
+    int64_t bytes = oa.bytes() + ob.bytes();
+    if (product == CCSP_OPS_BACK_WEIGHT) {
+        const int l = seg_log2_for<T>(n_rows, n_experts, out, inp);
+        if (l != 31) bytes += 2 * ((n_rows >> l) + 1) * part_floats(out, inp) * 4;
+    }
+    return bytes;
+}
+
+// the product's operands in their places, the rest of its arguments, the launch
+template <typename T, int PROD>
+int run_product(ProdArgs p, int64_t inp, int64_t out, const void* a, int64_t a_stride, const void* b, int64_t b_stride, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+    constexpr int product = PROD == PROD_FORWARD ? CCSP_OPS_FORWARD : (PROD == PROD_INPUT ? CCSP_OPS_BACK_INPUT : CCSP_OPS_BACK_WEIGHT);
+    const int64_t need = product_workspace<T>(product, p.E, p.R, inp, out, a, a_stride, b, b_stride);
+    CCSP_OPS_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "linear: workspace of %lld bytes is smaller than %lld or not aligned to 16 bytes",
+                   (long long)workspace_bytes, (long long)need);
+    char* ws = static_cast<char*>(workspace);
+    Operand<T> oa, ob;
+    linear_operands<T>(product, p.E, p.R, inp, out, a, a_stride, b, b_stride, &oa, &ob);
+    oa.place(&p.a, &p.lda, &ws, s);
+    ob.place(&p.b, &p.ldb, &ws, s);
+    p.b_expert = (PROD == PROD_WEIGHT ? 0 : out) * p.ldb;
+    p.parts = reinterpret_cast<float*>(ws);
+    p.quads = quads_ok<T>(p.N, p.ldc, p.c, p.z);
+    return launch_prod<T, PROD>(p, s);
 }

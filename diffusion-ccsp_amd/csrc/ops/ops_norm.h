@@ -82,7 +82,13 @@ __global__ __launch_bounds__(256) void k_norm_part(NormTable t, double* part) {
 __global__ __launch_bounds__(1024) void k_norm_finish(const double* part, long n, double max_norm, float* norm, float* scale) {
     __shared__ double sums[16];
     double s = 0.0;
-    for (long i = threadIdx.x; i < n; i += 1024) s += part[i];
+    for (long i = threadIdx.x; i < n; i += 16384) {              // sixteen loads in flight
+        double v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) v[u] = i + 1024 * u < n ? part[i + 1024 * u] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) s += v[u];
+    }
     s = sqrt(block_sum(s, sums, 16));
     if (threadIdx.x == 0) {
         norm[0] = (float)s;
@@ -122,7 +128,13 @@ __device__ __forceinline__ void clip_chunk(const T* p, T* o, long n, float c) {
         }
         done = head + nv * V;
     }
-    for (long t = done + threadIdx.x; t < n; t += 256) o[t] = (T)((float)p[t] * c);
+    for (long t = done + threadIdx.x; t < n; t += 2048) {        // (all of the chunk where the two are aligned differently)
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = t + 256 * u < n ? (float)p[t + 256 * u] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) if (t + 256 * u < n) o[t + 256 * u] = (T)(x[u] * c);
+    }
 }
 
 __global__ __launch_bounds__(256) void k_norm_clip(NormTable t, int blocks, const float* scale) {

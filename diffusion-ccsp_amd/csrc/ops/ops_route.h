@@ -8,11 +8,13 @@
 // depend on how the blocks run.
 //
 // A wave ranks 64 consecutive items at once: one ballot per key bit leaves the mask of the lanes that hold the same key, the bits
-// below the own lane are the rank, and a counter per (wave, key) in LDS carries from one step to the next.
+// below the own lane are the rank, and a counter per (wave, key) in LDS carries from one step to the next; at the end the counters are the wave's
+// counts.  (No LDS atomics: sorted ids, or one popular expert, would send all 64 lanes to one counter.)
 //
-// Two forms, by the number of assignments (both sides at the benchmark's ROUTE_SMALL limit are in the launch rule below): everything in
-// one block per sort and ONE launch, or three launches (count per tile, scan per key, place).  Keys of more than 4096 values (tokens) are
-// sorted by 12-bit digits, low digit first.
+// Latency bounds all of it: a plan of 40000 assignments is 1 MB.  So a thread loads the ids of all of its items at once and keeps the keys in registers
+// for the count and the rank.  Forms, by the number of assignments: everything in one block per sort and ONE launch; or two launches, count per tile and
+// place, where a placing block adds up the tiles before its own by itself; with many tiles a scan between them does that once.  Keys of more than
+// 4096 values (tokens) are sorted by 12-bit digits, low digit first.
 
 struct RouteIds {
     const void* expert;
@@ -37,8 +39,8 @@ __device__ __forceinline__ int route_key(const RouteIds& r, int by_token, int a)
 // one pass of one sort
 struct RoutePass {
     const int* in;          // items in their present order; null: 0, 1, 2, ...
-    int* out;               // items in their new order
-    int* hist;              // [bins][tiles], then totals [bins]
+    int* out;               // items in their new order (the expert sort leaves its result in RouteOut)
+    int* hist;              // [tiles][bins]; behind them, where a scan runs, totals [bins]
     int by_token, shift, bins, bits;
     int last;               // the pass that leaves the sorted order
 };
@@ -53,10 +55,12 @@ struct RouteOut {
 
 constexpr int ROUTE_TILE = 2048;                                 // items of a block: 4 waves x 8 steps x 64
 constexpr int ROUTE_BITS = 12, ROUTE_BINS = 1 << ROUTE_BITS;     // 4 waves x 4096 counters = 64 KB of LDS
+constexpr int ROUTE_PER = ROUTE_TILE / 256;                      // items of a thread
+constexpr int ROUTE_SCAN = 64;                                   // more reads of tile counts per thread of a placing block: a scan of its own
 constexpr int ROUTE_SMALL = 8192, ROUTE_SMALL_TOKENS = 16384;    // limits of the one-launch form
 constexpr int ROUTE_SMALL_BITS = 10;
 
-__device__ __forceinline__ int pass_digit(const RouteIds& r, const RoutePass& p, int a) { return (route_key(r, p.by_token, a) >> p.shift) & ((1 << p.bits) - 1); }
+__device__ __forceinline__ int pass_digit(const RoutePass& p, int key) { return (key >> p.shift) & ((1 << p.bits) - 1); }
 
 // rank of the lane's item among the lanes of the wave that hold the same digit (ascending lane), and the number of those lanes
 __device__ __forceinline__ int match_rank(int d, int bits, bool in, int* n) {
@@ -70,14 +74,23 @@ __device__ __forceinline__ int match_rank(int d, int bits, bool in, int* n) {
     return __popcll(m & ((1ull << lane) - 1));
 }
 
-// what the last pass of a sort leaves for item a at place pos
-__device__ __forceinline__ void route_place(const RouteIds& r, const RoutePass& p, const RouteOut& o, int a, int pos) {
-    p.out[pos] = a;
-    if (!p.last || p.by_token) return;
-    const bool in = route_key(r, 0, a) < r.E;
-    o.assign[pos] = in ? a : ~a;
-    o.rows[a] = in ? pos : -1;
-    o.row_token[pos] = in ? token_of(r, a) : -1;
+// PER steps of a wave: rank of every item among the wave's items of its digit; cnt (zeroed, the wave's own) becomes the wave's counts
+template <int PER>
+__device__ __forceinline__ void wave_ranks(const RoutePass& p, const int (&key)[PER], int (&rank)[PER], int* cnt, int steps) {
+#pragma unroll
+    for (int s = 0; s < PER; ++s) {
+        if (s >= steps) break;
+        const bool in = key[s] >= 0;
+        const int d = in ? pass_digit(p, key[s]) : 0;
+        int n;
+        const int r = match_rank(d, p.bits, in, &n);
+        // (atomic accesses: other lanes of the wave write a counter between a lane's reads of it)
+        const int base = in ? __hip_atomic_load(&cnt[d], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0;
+        __builtin_amdgcn_wave_barrier();                         // every lane has read before the first of a digit writes
+        if (in && r == 0) __hip_atomic_store(&cnt[d], base + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        __builtin_amdgcn_wave_barrier();
+        rank[s] = base + r;
+    }
 }
 
 // lower bound of key t in the sorted order
@@ -90,36 +103,44 @@ __device__ __forceinline__ int route_bound(const RouteIds& r, const int* order, 
     return lo;
 }
 
-// ---- three launches a pass -----------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void k_route_count(RouteIds r, RoutePass p0, RoutePass p1, int tiles) {
+// ---- several launches a pass ---------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_route_count(RouteIds r, RoutePass p0, RoutePass p1) {
     const RoutePass p = blockIdx.y ? p1 : p0;
     extern __shared__ int cnt[];
     for (int d = threadIdx.x; d < p.bins; d += 256) cnt[d] = 0;
-    __syncthreads();
-    const long i0 = (long)blockIdx.x * ROUTE_TILE;
-    for (int s = 0; s < ROUTE_TILE; s += 256) {
-        const long i = i0 + s + threadIdx.x;
-        if (i < r.A) atomicAdd(&cnt[pass_digit(r, p, p.in ? p.in[i] : (int)i)], 1);
+    const long i0 = (long)blockIdx.x * ROUTE_TILE + threadIdx.x;
+    int key[ROUTE_PER];
+#pragma unroll
+    for (int s = 0; s < ROUTE_PER; ++s) {
+        const long i = i0 + 256 * s;
+        key[s] = i < r.A ? route_key(r, p.by_token, p.in ? p.in[i] : (int)i) : -1;
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < p.bins; d += 256) p.hist[(size_t)d * tiles + blockIdx.x] = cnt[d];
+#pragma unroll
+    for (int s = 0; s < ROUTE_PER; ++s) {
+        const int d = key[s] >= 0 ? pass_digit(p, key[s]) : 0;
+        int n;
+        if (match_rank(d, p.bits, key[s] >= 0, &n) == 0 && key[s] >= 0) atomicAdd(&cnt[d], n);      // one lane per digit
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.bins; d += 256) p.hist[(size_t)blockIdx.x * p.bins + d] = cnt[d];
 }
 
-// a wave per digit: exclusive sum over the tiles, total behind
-__global__ __launch_bounds__(256) void k_route_scan(RoutePass p0, RoutePass p1, int tiles) {
+// a thread per digit: exclusive sum over the tiles, total behind
+__global__ __launch_bounds__(64) void k_route_scan(RoutePass p0, RoutePass p1, int tiles) {
     const RoutePass p = blockIdx.y ? p1 : p0;
-    const int d = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (d >= p.bins) return;
-    int* h = p.hist + (size_t)d * tiles;
+    const int d = blockIdx.x * 64 + threadIdx.x, bins = p.bins;
+    if (d >= bins) return;
     int run = 0;
-    for (int t0 = 0; t0 < tiles; t0 += 64) {
-        const int own = t0 + lane < tiles ? h[t0 + lane] : 0;
-        int v = own;
-        for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o); v += lane >= o ? u : 0; }
-        if (t0 + lane < tiles) h[t0 + lane] = run + v - own;
-        run += __shfl(v, 63);
+    for (int t = 0; t < tiles; t += 16) {
+        int c[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) c[u] = t + u < tiles ? p.hist[(size_t)(t + u) * bins + d] : 0;
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (t + u < tiles) { p.hist[(size_t)(t + u) * bins + d] = run; run += c[u]; }
     }
-    if (lane == 0) p.hist[(size_t)p.bins * tiles + d] = run;
+    p.hist[(size_t)tiles * bins + d] = run;
 }
 
 // exclusive sum over n values f(0) .. f(n - 1) by a block of NT threads, handed to g(i, sum); sums: one int per wave of LDS
@@ -139,38 +160,75 @@ __device__ __forceinline__ void block_exclusive(int n, int* sums, F f, G g) {
     __syncthreads();
 }
 
-__global__ __launch_bounds__(256) void k_route_place(RouteIds r, RoutePass p0, RoutePass p1, RouteOut o, int tiles) {
+__global__ __launch_bounds__(256) void k_route_place(RouteIds r, RoutePass p0, RoutePass p1, RouteOut o, int tiles, int scanned) {
     const RoutePass p = blockIdx.y ? p1 : p0;
-    extern __shared__ int cnt[];                                 // [4][bins]
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, bins = p.bins;
+    extern __shared__ int cnt[];                                 // [4][bins], then [bins]
     __shared__ int sums[4];
-    const int wave = threadIdx.x >> 6, bins = p.bins;
+    int* const start = cnt + 4 * bins;
     for (int d = threadIdx.x; d < 4 * bins; d += 256) cnt[d] = 0;
+    const long i0 = (long)blockIdx.x * ROUTE_TILE + wave * (ROUTE_TILE / 4) + lane;
+    int* const own = cnt + wave * bins;
+    int item[ROUTE_PER], key[ROUTE_PER], rank[ROUTE_PER];
+#pragma unroll
+    for (int s = 0; s < ROUTE_PER; ++s) {
+        const long i = i0 + 64 * s;
+        item[s] = i < r.A ? (p.in ? p.in[i] : (int)i) : -1;
+    }
+#pragma unroll
+    for (int s = 0; s < ROUTE_PER; ++s) key[s] = item[s] >= 0 ? route_key(r, p.by_token, item[s]) : -1;
     __syncthreads();
-    const long i0 = (long)blockIdx.x * ROUTE_TILE + wave * (ROUTE_TILE / 4) + (threadIdx.x & 63);
-    int* const cown = cnt + wave * bins;
-    volatile int* const own = cown;                              // (other lanes of the wave write it between a lane's reads)
-    for (int s = 0; s < ROUTE_TILE / 4; s += 64)
-        if (i0 + s < r.A) atomicAdd(&cown[pass_digit(r, p, p.in ? p.in[i0 + s] : (int)(i0 + s))], 1);
+    wave_ranks(p, key, rank, own, ROUTE_PER);
     __syncthreads();
-    const int* total = p.hist + (size_t)bins * tiles;
-    int* first = p.last ? (p.by_token ? (p.shift == 0 ? o.token_ptr : nullptr) : o.offsets) : nullptr;   // (one-pass sorts: the digit is the key)
-    block_exclusive<256>(bins, sums, [&](int d) { return total[d]; },
-        [&](int d, int start) {
-            if (first && blockIdx.x == 0) first[d] = start;      // (keys 0 .. E: the dropped ones start where the active rows end)
-            int run = start + p.hist[(size_t)d * tiles + blockIdx.x];
+    if (scanned) {                                               // start = the digit's total, counts = places inside the digit
+        for (int d0 = threadIdx.x; d0 < bins; d0 += 1024) {
+            int run[4], total[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int d = d0 + 256 * u;
+                run[u] = d < bins ? p.hist[(size_t)blockIdx.x * bins + d] : 0;
+                total[u] = d < bins ? p.hist[(size_t)tiles * bins + d] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int d = d0 + 256 * u;
+                if (d >= bins) break;
+                start[d] = total[u];
+                int at = run[u];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) { const int c = cnt[w * bins + d]; cnt[w * bins + d] = at; at += c; }
+            }
+        }
+    } else {
+        for (int d = threadIdx.x; d < bins; d += 256) {
+            int run = 0, total = 0;
+            for (int t = 0; t < tiles; t += 8) {
+                int c[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) c[u] = t + u < tiles ? p.hist[(size_t)(t + u) * bins + d] : 0;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) { total += c[u]; run += t + u < (int)blockIdx.x ? c[u] : 0; }
+            }
+            start[d] = total;
+#pragma unroll
             for (int w = 0; w < 4; ++w) { const int c = cnt[w * bins + d]; cnt[w * bins + d] = run; run += c; }
-        });
-    for (int s = 0; s < ROUTE_TILE / 4; s += 64) {
-        const bool in = i0 + s < r.A;
-        const int a = in ? (p.in ? p.in[i0 + s] : (int)(i0 + s)) : 0;
-        const int d = in ? pass_digit(r, p, a) : 0;
-        int n;
-        const int rank = match_rank(d, p.bits, in, &n);
-        const int base = in ? own[d] : 0;
-        __builtin_amdgcn_wave_barrier();
-        if (in && rank == 0) own[d] = base + n;
-        __builtin_amdgcn_wave_barrier();
-        if (in) route_place(r, p, o, a, base + rank);
+        }
+    }
+    __syncthreads();
+    block_exclusive<256>(bins, sums, [&](int d) { return start[d]; }, [&](int d, int first) { start[d] = first; });
+    int* first = !p.last ? nullptr : (p.by_token ? (p.shift == 0 ? o.token_ptr : nullptr) : o.offsets);      // (one-pass sorts: the digit is the key)
+    if (first && blockIdx.x == 0) for (int d = threadIdx.x; d < bins; d += 256) first[d] = start[d];         // (keys 0 .. E: the dropped ones start where the active rows end)
+#pragma unroll
+    for (int s = 0; s < ROUTE_PER; ++s) {
+        if (key[s] < 0) continue;
+        const int a = item[s], d = pass_digit(p, key[s]), pos = start[d] + own[d] + rank[s];
+        if (p.by_token || !p.last) p.out[pos] = a;
+        else {
+            const bool act = key[s] < r.E;
+            o.assign[pos] = act ? a : ~a;
+            o.rows[a] = act ? pos : -1;
+            o.row_token[pos] = act ? token_of(r, a) : -1;
+        }
     }
 }
 
@@ -186,55 +244,53 @@ __global__ __launch_bounds__(256) void k_route_zero(int* a, long na, int* b, lon
 }
 
 // ---- one launch: block 0 sorts by expert, block 1 (list tokens) by token -------------------------------------------------
-__global__ __launch_bounds__(512) void k_route_small(RouteIds r, RouteOut o, int* tmp0, int* tmp1, int expert_bits, int token_bits) {
+__global__ __launch_bounds__(512) void k_route_small(RouteIds r, RouteOut o, int* tmp, int expert_bits, int token_bits) {
+    constexpr int PER = ROUTE_SMALL / 512;                       // items of a thread
     extern __shared__ int cnt[];                                 // [8][bins]
     __shared__ int sums[8];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, by_token = blockIdx.x;
     const int key_bits = by_token ? token_bits : expert_bits;
     const int passes = by_token ? (key_bits + ROUTE_SMALL_BITS - 1) / ROUTE_SMALL_BITS : 1;
-    const int per = ((r.A + 511) / 512) * 64, i0 = wave * per + lane, i1 = wave * per + per < r.A ? wave * per + per : r.A;
+    const int steps = (r.A + 511) / 512, i0 = wave * steps * 64 + lane;      // a wave's run of items
     const int* in = nullptr;
     for (int ps = 0; ps < passes; ++ps) {
         RoutePass p;
-        p.in = in; p.by_token = by_token; p.shift = ps * ROUTE_SMALL_BITS;
+        p.shift = ps * ROUTE_SMALL_BITS;
         p.bits = by_token ? (key_bits - p.shift < ROUTE_SMALL_BITS ? key_bits - p.shift : ROUTE_SMALL_BITS) : key_bits;
-        p.bins = by_token ? 1 << p.bits : r.E + 1;
-        p.last = ps == passes - 1;
-        p.out = by_token ? (p.last ? o.token_assign : (ps & 1 ? tmp1 : tmp0)) : nullptr;
-        const int bins = p.bins;
-        int* const cown = cnt + wave * bins;
-        volatile int* const own = cown;
+        int* const out = ps == passes - 1 ? o.token_assign : tmp;            // (two passes at most: ROUTE_SMALL_TOKENS)
+        const int bins = by_token ? 1 << p.bits : r.E + 1;
+        int* const own = cnt + wave * bins;
         for (int d = threadIdx.x; d < 8 * bins; d += 512) cnt[d] = 0;
+        int item[PER], key[PER], rank[PER];
+#pragma unroll
+        for (int s = 0; s < PER; ++s) {
+            const int i = i0 + 64 * s;
+            item[s] = s < steps && i < r.A ? (in ? in[i] : i) : -1;
+        }
+#pragma unroll
+        for (int s = 0; s < PER; ++s) key[s] = item[s] >= 0 ? route_key(r, by_token, item[s]) : -1;
         __syncthreads();
-        for (int i = i0; i < i1; i += 64) atomicAdd(&cown[pass_digit(r, p, in ? in[i] : i)], 1);
+        wave_ranks(p, key, rank, own, steps);
         __syncthreads();
         block_exclusive<512>(bins, sums, [&](int d) { int c = 0; for (int w = 0; w < 8; ++w) c += cnt[w * bins + d]; return c; },
             [&](int d, int run) {
                 if (!by_token) o.offsets[d] = run;
                 for (int w = 0; w < 8; ++w) { const int c = cnt[w * bins + d]; cnt[w * bins + d] = run; run += c; }
             });
-        for (int i = i0; i < i0 - lane + per; i += 64) {          // (every lane of the wave in every step: the ballots are the wave's)
-            const bool live = i < i1;
-            const int a = live ? (in ? in[i] : i) : 0;
-            const int d = live ? pass_digit(r, p, a) : 0;
-            int n;
-            const int rank = match_rank(d, p.bits, live, &n);
-            const int base = live ? own[d] : 0;
-            __builtin_amdgcn_wave_barrier();
-            if (live && rank == 0) own[d] = base + n;
-            __builtin_amdgcn_wave_barrier();
-            if (live) {
-                if (by_token) p.out[base + rank] = a;
-                else {
-                    const bool act = d < r.E;
-                    o.assign[base + rank] = act ? a : ~a;
-                    o.rows[a] = act ? base + rank : -1;
-                    o.row_token[base + rank] = act ? token_of(r, a) : -1;
-                }
+#pragma unroll
+        for (int s = 0; s < PER; ++s) {
+            if (key[s] < 0) continue;
+            const int a = item[s], d = pass_digit(p, key[s]), pos = own[d] + rank[s];
+            if (by_token) out[pos] = a;
+            else {
+                const bool act = d < r.E;
+                o.assign[pos] = act ? a : ~a;
+                o.rows[a] = act ? pos : -1;
+                o.row_token[pos] = act ? token_of(r, a) : -1;
             }
         }
-        __syncthreads();                                         // (the block's own writes to p.out are the next pass's input)
-        in = p.out;
+        __syncthreads();                                         // (the block's own writes are the next pass's input)
+        in = out;
     }
     if (by_token)
         for (int t = threadIdx.x; t <= r.N; t += 512) o.token_ptr[t] = route_bound(r, o.token_assign, t);
@@ -242,38 +298,36 @@ __global__ __launch_bounds__(512) void k_route_small(RouteIds r, RouteOut o, int
 
 inline int bits_for(long keys) { int b = 0; while ((1l << b) < keys) ++b; return b; }        // digits that hold `keys` values
 
-// ints of workspace: histograms of the passes of both sorts (one at a time) and two orders between passes
+// ints of workspace: histograms of one pass of each sort, two orders between passes of the token sort
 inline size_t route_workspace_ints(long A, int E, long N, bool list) {
     const long tiles = cdiv(A, ROUTE_TILE);
     size_t w = (size_t)(E + 1) * (tiles + 1);
     if (list) {
         const int bits = bits_for(N + 1);
-        const long bins = bits > ROUTE_BITS ? ROUTE_BINS : N + 1;
-        w += (size_t)bins * (tiles + 1) + 2 * (size_t)A + (size_t)A;   // (+ the expert sort's own order)
-    } else w += (size_t)A;
+        w += (size_t)(bits > ROUTE_BITS ? ROUTE_BINS : N + 1) * (tiles + 1) + 2 * (size_t)A;
+    }
     return w;
 }
 
 int route(const RouteIds& r, const RouteOut& o, int* ws, hipStream_t s) {
     const bool list = o.token_ptr != nullptr;
     const int ebits = bits_for((long)r.E + 1), tbits = list ? bits_for((long)r.N + 1) : 0;
-    if (r.A == 0) {
-        // (nothing to sort: every first place is 0)
+    if (r.A == 0) {                                              // every first place is 0
         hipLaunchKernelGGL(k_route_zero, dim3((unsigned)cdiv((long)r.E + 1 + (list ? (long)r.N + 1 : 0), 256)), dim3(256), 0, s, o.offsets, r.E + 1, o.token_ptr, list ? r.N + 1 : 0);
         LAUNCHED();
         return 0;
     }
     if (r.A <= ROUTE_SMALL && (!list || r.N <= ROUTE_SMALL_TOKENS)) {
-        const int bins = list && (1 << ROUTE_SMALL_BITS) > r.E + 1 ? 1 << ROUTE_SMALL_BITS : r.E + 1;
-        hipLaunchKernelGGL(k_route_small, dim3(list ? 2 : 1), dim3(512), 8 * bins * sizeof(int), s, r, o, ws, ws + r.A, ebits, tbits);
+        const int token_bins = 1 << (tbits < ROUTE_SMALL_BITS ? tbits : ROUTE_SMALL_BITS), bins = list && token_bins > r.E + 1 ? token_bins : r.E + 1;
+        hipLaunchKernelGGL(k_route_small, dim3(list ? 2 : 1), dim3(512), 8 * bins * sizeof(int), s, r, o, ws, ebits, tbits);
         LAUNCHED();
         return 0;
     }
     const int tiles = (int)cdiv(r.A, ROUTE_TILE);
-    RoutePass pe = {nullptr, ws, ws + r.A, 0, 0, r.E + 1, ebits, 1}, pt = {};
-    int* w = ws + r.A + (size_t)(r.E + 1) * (tiles + 1);
+    const RoutePass pe = {nullptr, nullptr, ws, 0, 0, r.E + 1, ebits, 1};
+    RoutePass pt = {};
     const int tpasses = list ? (int)cdiv(tbits, ROUTE_BITS) : 0;
-    int *tmp0 = w, *tmp1 = w + r.A, *thist = w + 2 * (size_t)r.A;
+    int *tmp0 = ws + (size_t)(r.E + 1) * (tiles + 1), *tmp1 = tmp0 + r.A, *thist = tmp1 + r.A;
     const int* tin = nullptr;
     for (int ps = 0; ps < (tpasses > 1 ? tpasses : 1); ++ps) {
         int jobs = ps == 0 ? 1 : 0;
@@ -288,9 +342,10 @@ int route(const RouteIds& r, const RouteOut& o, int* ws, hipStream_t s) {
         }
         const RoutePass& a = ps == 0 ? pe : pt;                  // (the expert sort is one pass: it runs beside the tokens' first)
         const int bins = jobs == 2 && pt.bins > pe.bins ? pt.bins : a.bins;
-        hipLaunchKernelGGL(k_route_count, dim3(tiles, jobs), dim3(256), bins * sizeof(int), s, r, a, pt, tiles);
-        hipLaunchKernelGGL(k_route_scan, dim3((unsigned)cdiv(bins, 4), jobs), dim3(256), 0, s, a, pt, tiles);
-        hipLaunchKernelGGL(k_route_place, dim3(tiles, jobs), dim3(256), 4 * bins * sizeof(int), s, r, a, pt, o, tiles);
+        const int scan = tiles * cdiv(bins, 256) > ROUTE_SCAN;
+        hipLaunchKernelGGL(k_route_count, dim3(tiles, jobs), dim3(256), bins * sizeof(int), s, r, a, pt);
+        if (scan) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)cdiv(bins, 64), jobs), dim3(64), 0, s, a, pt, tiles);
+        hipLaunchKernelGGL(k_route_place, dim3(tiles, jobs), dim3(256), 5 * bins * sizeof(int), s, r, a, pt, o, tiles, scan);
     }
     if (tpasses > 1) hipLaunchKernelGGL(k_route_ptr, dim3((unsigned)cdiv((long)r.N + 1, 256)), dim3(256), 0, s, r, o.token_assign, o.token_ptr);
     LAUNCHED();

@@ -48,6 +48,7 @@ __global__ __launch_bounds__(256) void k_rows_combine(long n_tokens, int chunks,
                                                       const int* __restrict__ rows, const void* __restrict__ w, int wf32, const T* __restrict__ src, long src_stride,
                                                       T* __restrict__ dst, long dst_stride) {
     typedef typename VecOf<T, V>::type VT;
+    constexpr int U = 8;
     const int tpr = 1 << tpr_log2, rpb = 256 >> tpr_log2;
     const long n = block_id() * rpb + (threadIdx.x >> tpr_log2);
     if (n >= n_tokens) return;
@@ -56,12 +57,12 @@ __global__ __launch_bounds__(256) void k_rows_combine(long n_tokens, int chunks,
         float acc[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-        for (long j = j0; j < j1; j += 4) {                      // four rows in flight
-            VT v[4];
-            float wt[4];
-            int row[4];
+        for (long j = j0; j < j1; j += U) {                      // U rows in flight
+            VT v[U];
+            float wt[U];
+            int row[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 row[u] = -1; wt[u] = 0.0f;
                 if (j + u < j1) {
                     const int a = token_ptr ? token_assign[j + u] : (int)(j + u);
@@ -70,10 +71,10 @@ __global__ __launch_bounds__(256) void k_rows_combine(long n_tokens, int chunks,
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
                 if (row[u] >= 0) v[u] = *reinterpret_cast<const VT*>(src + row[u] * src_stride + (long)c * V);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
                 if (row[u] >= 0) {                               // (a dropped assignment adds nothing, not 0 x something)
                     const T* e = reinterpret_cast<const T*>(&v[u]);
 #pragma unroll

@@ -199,15 +199,28 @@ def combine_rows(ys, plan, weights=None):
     return _CombineRows.apply(ys, weights, plan)
 
 
+def _linear_space(product, code, E, plan, I, O, a, b):
+    """(address, bytes, the tensor that holds them) of a product's workspace; a, b: its operands"""
+    need = _ops.lib().ccsp_ops_linear_workspace(product, code, E, plan.n_rows, I, O, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(-2))
+    if need < 0:
+        raise ValueError('expert_linear: %d rows, %d -> %d of %d experts are out of range' % (plan.n_rows, I, O, E))
+    if need == 0:
+        return None, 0, None
+    ws = torch.empty(need, dtype=torch.uint8, device=a.device)
+    return ws.data_ptr(), need, ws
+
+
 class _ExpertLinear(Function):
     @staticmethod
     def forward(ctx, xs, weight, bias, plan, act):
         x = _rows(xs)
         E, O, I = weight.shape
+        code = _TYPE[x.dtype]
         y = torch.empty((plan.n_rows, O), dtype=x.dtype, device=x.device)
         z = torch.empty_like(y) if act and any(ctx.needs_input_grad) else None
-        _run(x.device, _ops.lib().ccsp_ops_linear, _TYPE[x.dtype], E, plan.n_rows, I, O, plan.offsets.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(),
-             None if bias is None else bias.data_ptr(), act, y.data_ptr(), None if z is None else z.data_ptr())
+        at, need, ws = _linear_space(0, code, E, plan, I, O, x, weight)
+        _run(x.device, _ops.lib().ccsp_ops_linear, code, E, plan.n_rows, I, O, plan.offsets.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(),
+             None if bias is None else bias.data_ptr(), act, y.data_ptr(), None if z is None else z.data_ptr(), at, need)
         ctx.plan, ctx.act = plan, act
         ctx.save_for_backward(x if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None, weight, z)
         return y
@@ -228,16 +241,16 @@ class _ExpertLinear(Function):
         d_x = d_w = d_b = None
         if ctx.needs_input_grad[0]:
             d_x = torch.empty((plan.n_rows, I), dtype=g.dtype, device=dev)
-            _run(dev, L.ccsp_ops_linear_back_input, code, E, plan.n_rows, I, O, off, dz.data_ptr(), dz.stride(0), weight.data_ptr(), d_x.data_ptr())
+            at, need, ws = _linear_space(1, code, E, plan, I, O, dz, weight)
+            _run(dev, L.ccsp_ops_linear_back_input, code, E, plan.n_rows, I, O, off, dz.data_ptr(), dz.stride(0), weight.data_ptr(), d_x.data_ptr(), at, need)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             if ctx.needs_input_grad[1]:
                 d_w = torch.empty((E, O, I), dtype=g.dtype, device=dev)
             if ctx.needs_input_grad[2]:
                 d_b = torch.empty((E, O), dtype=g.dtype, device=dev)
-            need = L.ccsp_ops_linear_back_weight_workspace(code, E, plan.n_rows, I, O)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            at, need, ws = _linear_space(2, code, E, plan, I, O, dz, x)
             _run(dev, L.ccsp_ops_linear_back_weight, code, E, plan.n_rows, I, O, off, dz.data_ptr(), dz.stride(0), x.data_ptr(), x.stride(0),
-                 None if d_w is None else d_w.data_ptr(), None if d_b is None else d_b.data_ptr(), ws.data_ptr(), need)
+                 None if d_w is None else d_w.data_ptr(), None if d_b is None else d_b.data_ptr(), at, need)
         return d_x, d_w, d_b, None, None
 
 

@@ -31,7 +31,8 @@ enum { CCSP_OPS_NONE = 0, CCSP_OPS_SILU = 1 };
 
 #define CCSP_OPS_MAX_ASSIGN (1 << 30)     /* assignments, rows, tokens */
 #define CCSP_OPS_MAX_EXPERTS 1024
-#define CCSP_OPS_MAX_WIDTH (1 << 24)
+#define CCSP_OPS_MAX_WIDTH (1 << 24)      /* elements of a row that is moved */
+#define CCSP_OPS_MAX_FEATURES (1 << 20)   /* inputs, outputs of an expert */
 
 int32_t ccsp_ops_version(void);           /* major * 1000 + minor */
 const char* ccsp_ops_last_error(void);
@@ -63,18 +64,22 @@ int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_
 
 /* The experts' products.  Rows offsets[e] .. offsets[e + 1] - 1 belong to expert e; weight [n_experts, out, inp] and bias [n_experts, out] (NULL: none) are
  * contiguous.  y = act(x weight[e]^T + bias[e]) [n_rows, out] contiguous, zeros in the rows behind offsets[n_experts].  z, where not NULL, receives the
- * pre-activation of the active rows (what silu_back reads).  Products and sums in 32 bits. */
+ * pre-activation of the active rows (what silu_back reads).  Products and sums in 32 bits.
+ * workspace (each of the three products): ccsp_ops_linear_workspace bytes, aligned to 16, for the same operands: copies of operands whose rows are not whole
+ * 16-byte pieces at multiples of 16 bytes, and partial sums of the weight gradient.  Often 0; -1: an argument is out of range. */
+enum { CCSP_OPS_FORWARD = 0 /* a = x, b = weight */, CCSP_OPS_BACK_INPUT = 1 /* a = dz, b = weight */, CCSP_OPS_BACK_WEIGHT = 2 /* a = dz, b = x */ };
+int64_t ccsp_ops_linear_workspace(int32_t product, int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const void* a, int64_t a_stride, const void* b,
+                                  int64_t b_stride);
 int ccsp_ops_linear(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* x, int64_t x_stride, const void* weight,
-                    const void* bias, int32_t activation, void* y, void* z, void* stream);
+                    const void* bias, int32_t activation, void* y, void* z, void* workspace, int64_t workspace_bytes, void* stream);
 /* dz = dy * silu'(z) in the active rows; the rows behind are not written. */
 int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, int64_t out, const int32_t* offsets, const void* dy, int64_t dy_stride, const void* z, void* dz,
                               void* stream);
 /* dx = dz weight[e] [n_rows, inp], zeros behind the last active row. */
 int ccsp_ops_linear_back_input(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride,
-                               const void* weight, void* dx, void* stream);
+                               const void* weight, void* dx, void* workspace, int64_t workspace_bytes, void* stream);
 /* d_weight[e] = sum over the expert's rows of dz^T x, d_bias[e] = sum of dz; zeros for an expert without rows.  Either may be
- * NULL; d_bias has the same bits with and without d_weight.  workspace: ccsp_ops_linear_back_weight_workspace bytes (may be 0), aligned to 16. */
-int64_t ccsp_ops_linear_back_weight_workspace(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out);
+ * NULL; d_bias has the same bits with and without d_weight. */
 int ccsp_ops_linear_back_weight(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* dz, int64_t dz_stride, const void* x,
                                 int64_t x_stride, void* d_weight, void* d_bias, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -92,14 +92,16 @@ def test_c_entries_refuse_before_any_launch():
     refused(L.ccsp_ops_rows_gather(0, -1, 4, ok, 4, ok, ok, None), 'range')
     refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, ok, 2, ok, 4, ok, None), 'weights')
     refused(L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, 2, ok, 4, ok, 4, ok, ok, None), 'weights')
-    refused(L.ccsp_ops_linear(0, 4, 4, 0, 4, ok, ok, 4, ok, None, 0, ok, None, None), 'range')
-    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, ok, None, 5, ok, None, None), 'activation')
-    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, None, ok, 4, ok, None, 0, ok, None, None), 'null')
-    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, None, None, 0, ok, None, None), 'null')
-    refused(L.ccsp_ops_linear_back_input(0, 4, 4, 4, 4, ok, ok, 4, None, ok, None), 'null')
+    refused(L.ccsp_ops_linear(0, 4, 4, 0, 4, ok, ok, 4, ok, None, 0, ok, None, None, 0, None), 'range')
+    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, ok, None, 5, ok, None, None, 0, None), 'activation')
+    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, None, ok, 4, ok, None, 0, ok, None, None, 0, None), 'null')
+    refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, None, None, 0, ok, None, None, 0, None), 'null')
+    refused(L.ccsp_ops_linear(0, 4, 4, 5, 4, ok, ok, 5, ok, None, 0, ok, None, None, 0, None), 'workspace')
+    refused(L.ccsp_ops_linear_back_input(0, 4, 4, 4, 4, ok, ok, 4, None, ok, None, 0, None), 'null')
     refused(L.ccsp_ops_linear_back_weight(0, 4, 4, 4, 4, ok, ok, 4, ok, 4, None, None, ok, 64, None), 'null')
     refused(L.ccsp_ops_linear_back_weight(0, 2, 2000, 4, 4, ok, ok, 4, ok, 4, ok, None, ok, 64, None), 'workspace')
-    assert L.ccsp_ops_linear_back_weight_workspace(0, 2, 2000, 0, 4) == -1
+    assert L.ccsp_ops_linear_workspace(2, 0, 2, 2000, 0, 4, ok, 4, ok, 4) == -1 and L.ccsp_ops_linear_workspace(3, 0, 2, 8, 4, 4, ok, 4, ok, 4) == -1
+    assert L.ccsp_ops_linear_workspace(0, 0, 2, 8, 4, 4, ok, 4, ok, 4) == 0 and L.ccsp_ops_linear_workspace(0, 0, 2, 8, 4, 4, ok, 5, ok, 4) == 256
     refused(L.ccsp_ops_linear_silu_back(0, 4, 4, 4, ok, ok, 4, None, ok, None), 'null')
     sizes, types, ptrs = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(0), (ctypes.c_void_p * 1)(64)
     refused(L.ccsp_ops_clip_norm(1, ptrs, ptrs, sizes, types, -1.0, ok, ok, ok, 64, None), 'negative')
@@ -250,6 +252,8 @@ def strided(t, how, device):
     t = t.to(device)
     if how == 'plain':
         return t
+    if how == 'expanded':                                         # every row the first one
+        return t[:1].expand(t.shape)
     wide = torch.full((t.shape[0], t.shape[1] + 3), float('nan'), dtype=t.dtype, device=device)
     wide[:, 1:1 + t.shape[1]] = t
     if how == 'offset':
@@ -406,6 +410,24 @@ def test_expert_linear_on_strided_rows(device, layout, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', list(DTYPES))
+def test_expert_linear_of_rows_that_are_one_row(device, dtype):
+    """inputs and gradients broadcast over the rows: the same bits as their copies"""
+    dt = DTYPES[dtype]
+    expert, xs, w, bias, gy = linear_case([70, 0, 90], 2, 64, 96, dt, 4)
+    plan = ops.route(expert.to(device), 3)
+    out = []
+    for how in ('expanded', 'plain'):
+        x, g = strided(xs, 'expanded', device), strided(gy, 'expanded', device)
+        if how == 'plain':
+            x, g = x.contiguous(), g.contiguous()
+        x, wd, bd = x.requires_grad_(), w.to(device).requires_grad_(), bias.to(device).requires_grad_()
+        y = ops.expert_linear(x, wd, plan, bd)
+        out.append([y.detach()] + list(torch.autograd.grad(y, [x, wd, bd], g)))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES))
 def test_expert_linear_of_many_experts(device, dtype):
     """more experts than a wave has lanes, most of them empty; a long group that ends inside a tile"""
     counts = [(3 * e) % 5 if e % 7 else 0 for e in range(201)]
@@ -418,7 +440,7 @@ def test_expert_linear_of_many_experts(device, dtype):
 @pytest.mark.parametrize('dtype', list(DTYPES))
 def test_expert_linear_with_rows_cut_into_segments(device, counts, dtype):
     """experts longer than a segment of the weight gradient, at its border, and without rows beside them"""
-    need = _ops.lib().ccsp_ops_linear_back_weight_workspace(_ops.TYPES[str(DTYPES[dtype])[6:]], len(counts), sum(counts), 24, 40)
+    need = _ops.lib().ccsp_ops_linear_workspace(2, _ops.TYPES[str(DTYPES[dtype])[6:]], len(counts), sum(counts), 24, 40, 64, 40, 64, 24)
     assert need > 0
     check_linear(device, counts, 3, 24, 40, DTYPES[dtype], 'silu', True)
     check_linear(device, counts, 0, 23, 41, DTYPES[dtype], None, True)
