@@ -497,6 +497,20 @@ def test_a_frozen_weight_or_input_gets_no_gradient(device):
         assert torch.equal(got, want[i])
 
 
+@pytest.mark.gpu
+def test_a_gradient_of_a_gradient_is_refused(device):
+    expert, leaves, E = layer_inputs(device, torch.float32)
+    plan = ops.route(expert, E)
+    x = leaves[0].requires_grad_()
+    w = leaves[1].requires_grad_()
+    rows = ops.sort_rows(x, plan)
+    for y in (rows, ops.expert_linear(rows.detach().requires_grad_(), w, plan), ops.combine_rows(rows, plan, leaves[4].requires_grad_())):
+        leaf = x if y is rows else w if y.shape[1] == w.shape[1] else leaves[4]
+        g, = torch.autograd.grad(y.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match='differentiable once'):
+            g.sum().backward()
+
+
 # ---- the global norm -----------------------------------------------------------------------------------------------------
 
 def norm_oracle(ts, max_norm):
