@@ -20,7 +20,7 @@ struct ProdArgs {
     const int* offsets;
     int E, R, M, N, K;                                           // M, N, K of one expert's product; the one that is a row count is -1
     int silu;
-    int quads;                                                   // rows of the result take four elements at once: their number, stride and addresses are multiples
+    int pieces;                                                  // elements of a result's row that one access may take: 8, 4 or 1
     float* parts;                                                // weight gradient of experts with more than 2^seg_log2 rows: [slot][M N + M] partial sums
     int seg_log2;                                                // 31: no expert's rows are cut
 };
@@ -59,9 +59,30 @@ __device__ __forceinline__ int count_tiles(const int* __restrict__ off, int E, i
 // most tiles of 2^l rows that R rows in E groups and a tail can have
 inline long most_tiles(long R, long E, int l) { const long g = R < E + 1 ? R : E + 1; return (R >> l) + g; }
 
-__device__ __forceinline__ float silu_value(float z) { return z / (1.0f + expf(-z)); }
-__device__ __forceinline__ float silu_slope(float z) { const float s = 1.0f / (1.0f + expf(-z)); return s * (1.0f + z * (1.0f - s)); }
+// sigmoid: in 32 bits by expf and a true division; for results of 16 bits by the hardware's exponential and reciprocal, whose 2^-22 is a thousandth of the
+// result's own rounding and whose few instructions an epilogue notices (8192 rows, 32 experts of 2048 -> 1408: the forward product 115 -> 77 us)
+template <typename T> __device__ __forceinline__ float sigmoid_of(float z) {
+    if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+template <typename T> __device__ __forceinline__ float silu_value(float z) { return sizeof(T) == 4 ? z / (1.0f + expf(-z)) : z * sigmoid_of<T>(z); }
+template <typename T> __device__ __forceinline__ float silu_slope(float z) { const float s = sigmoid_of<T>(z); return s * (1.0f + z * (1.0f - s)); }
 
+// s + the eight values of v, in 32 bits
+__device__ __forceinline__ float add_all(__attribute__((ext_vector_type(8))) bf16 v, float s) {
+    typedef bf16 V2 __attribute__((ext_vector_type(2)));
+    const V2 one = {(bf16)1.0f, (bf16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(V2{v[i], v[i + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float add_all(__attribute__((ext_vector_type(8))) fp16 v, float s) {
+    typedef fp16 V2 __attribute__((ext_vector_type(2)));
+    const V2 one = {(fp16)1.0f, (fp16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(V2{v[i], v[i + 1]}, one, s, false);
+    return s;
+}
 template <typename T> struct Vec8 { typedef T t __attribute__((ext_vector_type(8))); };
 __device__ __forceinline__ f32x4 mfma16(Vec8<bf16>::t a, Vec8<bf16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma16(Vec8<fp16>::t a, Vec8<fp16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -194,6 +215,17 @@ __host__ __device__ __forceinline__ int seg_slot(int first, int i, int l) { retu
 // a slot: the product, the sums, rounded up to 16 bytes
 __host__ __device__ __forceinline__ long part_floats(long M, long N) { return (M * N + M + 3) & ~3l; }
 
+// asks the scheduler for LDS reads and matrix instructions in turn, R reads spread over M
+template <int R, int M, int I = 0>
+__device__ __forceinline__ void spread_reads() {
+    if constexpr (I < R) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       // one LDS read
+        constexpr int n = (I + 1) * M / R - I * M / R;
+        if constexpr (n > 0) __builtin_amdgcn_sched_group_barrier(0x008, n, 0);
+        spread_reads<R, M, I + 1>();
+    }
+}
+
 template <int V> struct Log2 { static constexpr int v = 1 + Log2<V / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
@@ -202,7 +234,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     constexpr bool AKC = PROD != PROD_WEIGHT, BKC = PROD == PROD_FORWARD, F32 = sizeof(T) == 4;
     constexpr int G = F32 ? 32 : 16, FA = TM / WM / G, FB = TN / WN / G, RG = F32 ? 16 : 4;      // fragment side, fragments, result registers
     constexpr int SK = 128 / sizeof(T), STAGE = (TM + TN) * SK;
+    constexpr int KS = F32 ? 4 : 2;                              // k steps of a stage
     typedef typename VecOf<float, RG>::type Acc;
+    typedef typename std::conditional<F32, f32x4, typename Vec8<T>::t>::type Frag;
     extern __shared__ __attribute__((aligned(16))) unsigned short lds[];
     const T* const sm = reinterpret_cast<const T*>(lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
@@ -231,75 +265,117 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     const T* A = static_cast<const T*>(p.a) + (PROD == PROD_WEIGHT ? (long)r0 * p.lda + m0 : (long)r0 * p.lda);
     const T* B = static_cast<const T*>(p.b) + (PROD == PROD_WEIGHT ? (long)r0 * p.ldb + n0 : e * p.b_expert + (BKC ? (long)n0 * p.ldb : (long)n0));
     Acc acc[FA][FB] = {};
-    // the bias gradient (sum over k of A) is made on the way by the waves that hold the first columns of n: in 16 bits a product with a column of ones,
-    // in 32 bits one addition beside each 64-cycle matrix instruction
+    // the bias gradient (sum over k of A) is made on the way by the waves that hold the first columns of n: vector additions beside the matrix
+    // instructions, each lane over the k that it holds
     const bool sums = PROD == PROD_WEIGHT && p.sum && n0 + wn == 0;
-    f32x4 sum16[FA] = {};
-    float sum32[FA] = {};
+    float sum[FA] = {};
+    // 32 bits: a chain of K additions into one register would lose sqrt(K) roundings' worth; every FLUSH stages it goes into a second one
+    constexpr int FLUSH = 4;
+    Acc total[F32 ? FA : 1][F32 ? FB : 1] = {};
+    float total_sum[F32 ? FA : 1] = {};
     if (K > 0) {
         Stager<T, AKC, TM, WM * WN> ga;
         Stager<T, BKC, TN, WM * WN> gb;
         ga.init(A, p.lda, left_m);
         gb.init(B, p.ldb, N - n0);
         const unsigned int l0 = (unsigned int)(unsigned long)(__attribute__((address_space(3))) unsigned short*)lds;
-        constexpr int BYTES = STAGE * (int)sizeof(T), LOADS = (NST - 2) * (ga.N + gb.N);        // of a stage; of the stages that may be on their way
-        static_assert(LOADS < 64, "the wait's counter");
+        constexpr int BYTES = STAGE * (int)sizeof(T), L = ga.N + gb.N;       // of a stage; a wave's loads for it
+        static_assert((NST - 1) * L < 64, "the wait's counter");
+        const int stages = (K + SK - 1) / SK;
+        auto fetch = [&](int st, int buf) {
+            ga.load(l0 + buf * BYTES, K - st * SK);
+            gb.load(l0 + buf * BYTES + TM * 128, K - st * SK);
+        };
 #pragma unroll
-        for (int i = 0; i < NST - 1; ++i)
-            if (i * SK < K) { ga.load(l0 + i * BYTES, K - i * SK); gb.load(l0 + i * BYTES + TM * 128, K - i * SK); }
+        for (int i = 0; i < NST; ++i) if (i < stages) fetch(i, i);
+        // A wave multiplies one k step while the next one's fragments come out of LDS; at a stage's last step those are the next stage's, so that is where it
+        // has to be there.  Its loads come back in order: NST - 2 later stages may still be on their way.  The barrier makes it everyone's part of
+        // the stage, and says that nobody reads this stage any more (its reads have come back): the loads for the stage NST further go into its place.
+        Frag fa[2][FA], fb[2][FB];
+        constexpr int ACROSS = F32 ? 4 : 2, READS = FA * (AKC ? 1 : ACROSS) + FB * (BKC ? 1 : ACROSS);       // LDS reads of a k step
+        auto read = [&](int set, int buf, int ks) {
+            const T *sA = sm + buf * STAGE, *sB = sA + TM * SK;
+#pragma unroll
+            for (int j = 0; j < FB; ++j) {
+                if constexpr (F32) fb[set][j] = stage_frag32<BKC, TN>(sB, wn + G * j, ks);
+                else fb[set][j] = stage_frag<T, BKC, TN>(sB, wn + G * j, ks);
+            }
+#pragma unroll
+            for (int i = 0; i < FA; ++i) {
+                if constexpr (F32) fa[set][i] = stage_frag32<AKC, TM>(sA, wm + G * i, ks);
+                else fa[set][i] = stage_frag<T, AKC, TM>(sA, wm + G * i, ks);
+            }
+        };
         auto loop = [&](auto with_sums) {
             constexpr bool S = decltype(with_sums)::value;
-            int buf = 0;
-            for (int k0 = 0; k0 < K; k0 += SK, buf = buf + 1 == NST ? 0 : buf + 1) {
-                // this wave's part of the stage is there (its loads come back in order, NST - 2 later stages may be on their way);
-                if (k0 + (NST - 2) * SK < K) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();                    // everyone's, and nobody reads the stage before it any more (its reads have come back)
-                asm volatile("" ::: "memory");
-                if (k0 + (NST - 1) * SK < K) {
-                    const unsigned int l1 = l0 + (buf == 0 ? NST - 1 : buf - 1) * BYTES;
-                    ga.load(l1, K - k0 - (NST - 1) * SK);
-                    gb.load(l1 + TM * 128, K - k0 - (NST - 1) * SK);
-                }
-                const T *sA = sm + buf * STAGE, *sB = sA + TM * SK;
-                if constexpr (F32) {
+            auto multiply = [&](int set) {
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        f32x4 fa[FA], fb[FB];
+                for (int k = 0; k < (F32 ? 4 : 1); ++k)
 #pragma unroll
-                        for (int j = 0; j < FB; ++j) fb[j] = stage_frag32<BKC, TN>(sB, wn + G * j, ks);
+                    for (int i = 0; i < FA; ++i) {
 #pragma unroll
-                        for (int i = 0; i < FA; ++i) fa[i] = stage_frag32<AKC, TM>(sA, wm + G * i, ks);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-#pragma unroll
-                            for (int i = 0; i < FA; ++i) {
-#pragma unroll
-                                for (int j = 0; j < FB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][k], fa[i][k], acc[i][j], 0, 0, 0);
-                                if (S) sum32[i] += fa[i][k];
-                            }
+                        for (int j = 0; j < FB; ++j) {
+                            if constexpr (F32) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[set][j][k], fa[set][i][k], acc[i][j], 0, 0, 0);
+                            else acc[i][j] = mfma16(fb[set][j], fa[set][i], acc[i][j]);
+                        }
+                        if constexpr (F32) { if (S) sum[i] += fa[set][i][k]; }
                     }
-                } else {
+                if constexpr (!F32) if (S) {
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int ks = 0; ks < 2; ++ks) {
-                        typename Vec8<T>::t fa[FA], fb[FB], ones;
+                    for (int i = 0; i < FA; ++i) sum[i] = add_all(fa[set][i], sum[i]);
+                }
+            };
+            if (NST <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            // (the sums' registers and a second set of fragments do not fit beside a 128 x 64 part: there a step waits for its own fragments)
+            constexpr bool AHEAD = !(S && TM == 256);
+            if (AHEAD) read(0, 0, 0);
+            int buf = 0;
+            for (int st = 0; st < stages; ++st) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) ones[i] = (T)1.0f;
-#pragma unroll
-                        for (int j = 0; j < FB; ++j) fb[j] = stage_frag<T, BKC, TN>(sB, wn + G * j, ks);
-#pragma unroll
-                        for (int i = 0; i < FA; ++i) fa[i] = stage_frag<T, AKC, TM>(sA, wm + G * i, ks);
+                for (int ks = 0; ks < KS - 1; ++ks) {
+                    if (AHEAD) read((ks + 1) & 1, buf, ks + 1); else read(0, buf, ks);
+                    multiply(AHEAD ? ks & 1 : 0);
+                    if (AHEAD) spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
+                }
+                if (!AHEAD) { read(0, buf, KS - 1); multiply(0); }
+                if (st + NST - 1 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * L) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (st + NST < stages) fetch(st + NST, buf);
+                buf = buf + 1 == NST ? 0 : buf + 1;
+                if (AHEAD) {
+                    read(0, buf, 0);                             // (behind the last stage: whatever lies there, unused)
+                    asm volatile("" ::: "memory");               // (or the compiler reads them in the next round after all)
+                    multiply((KS - 1) & 1);
+                    spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
+                }
+                if constexpr (F32) {
+                    if ((st + 1) % FLUSH == 0) {
+                        asm volatile("" ::: "memory");          // (a branch, not 48 selects every stage)
 #pragma unroll
                         for (int i = 0; i < FA; ++i) {
 #pragma unroll
-                            for (int j = 0; j < FB; ++j) acc[i][j] = mfma16(fb[j], fa[i], acc[i][j]);
-                            if (S) sum16[i] = mfma16(ones, fa[i], sum16[i]);
+                            for (int j = 0; j < FB; ++j) { total[i][j] += acc[i][j]; acc[i][j] = Acc{}; }
+                            if (S) { total_sum[i] += sum[i]; sum[i] = 0.0f; }
                         }
                     }
                 }
             }
         };
         if (PROD == PROD_WEIGHT && sums) loop(std::true_type{}); else loop(std::false_type{});
+    }
+    if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i) {
+#pragma unroll
+            for (int j = 0; j < FB; ++j) acc[i][j] += total[i][j];
+            sum[i] += total_sum[i];
+        }
     }
     typedef typename VecOf<T, 4>::type V4;
     T* C = static_cast<T*>(p.c) + (PROD == PROD_WEIGHT ? e * p.c_expert + (long)m0 * p.ldc : (long)r0 * p.ldc);
@@ -309,7 +385,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     if (sums) {
 #pragma unroll
         for (int i = 0; i < FA; ++i) {
-            const float v = F32 ? sum32[i] + __shfl_xor(sum32[i], 32) : sum16[i][0];
+            float v = sum[i] + __shfl_xor(sum[i], 32);           // (the lanes of a row hold its k between them)
+            if (!F32) v += __shfl_xor(v, 16);
             const int m = wm + G * i + lane;
             if (lane < G && m < left_m) {
                 if (part) part[(long)p.M * p.N + m0 + m] = v; else static_cast<T*>(p.sum)[(long)e * p.M + m0 + m] = (T)v;
@@ -317,6 +394,49 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
         }
     }
     if (PROD == PROD_WEIGHT && !p.c) return;                     // (the sums alone)
+    if constexpr (!F32) {
+        // Whole 16-byte pieces: the wave's part goes through its share of LDS (free since the last barrier), so that a store writes eight rows' runs of
+        // 16 (TN / WN) / 8 bytes instead of sixteen rows' 32: 65536 rows, 16 experts 2048 -> 4096: 1220 -> 1080 us
+        if (p.pieces == 8 && !part) {
+            constexpr int PM = TM / WM, PN = TN / WN, CH = PN / 8;         // the wave's part, 16-byte pieces of its row
+            T* const own = reinterpret_cast<T*>(lds) + wave * PM * PN;
+            static_assert(WM * WN * PM * PN * 2 <= NST * (TM + TN) * 128, "the parts fit");
+            f32x4 bv[FB];
+#pragma unroll
+            for (int j = 0; j < FB; ++j) {
+                const int n = n0 + wn + G * j + 4 * (lane >> 4);
+                bv[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (bias && n < N) {
+                    const V4 b = *reinterpret_cast<const V4*>(bias + n);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) bv[j][r] = (float)b[r];
+                }
+            }
+            auto out = [&](T* to, bool act) {
+#pragma unroll
+                for (int i = 0; i < FA; ++i)
+#pragma unroll
+                    for (int j = 0; j < FB; ++j) {
+                        const int m = G * i + (lane & 15), c = 2 * j + (lane >> 5);
+                        V4 y;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) { const float v = acc[i][j][r] + bv[j][r]; y[r] = act ? (T)silu_value<T>(v) : (T)v; }
+                        *reinterpret_cast<V4*>(own + m * PN + ((c ^ (m & (CH - 1))) << 3) + 4 * (lane >> 4 & 1)) = y;
+                    }
+                asm volatile("" ::: "memory");                   // (a wave's LDS accesses keep their order; other lanes wrote what a lane reads)
+#pragma unroll
+                for (int it = 0; it < PM * CH / 64; ++it) {
+                    const int m = it * (64 / CH) + lane / CH, c = lane % CH, n = n0 + wn + 8 * c;
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(own + m * PN + ((c ^ (m & (CH - 1))) << 3));
+                    if (wm + m < left_m && n < N) *reinterpret_cast<u32x4*>(to + (long)(wm + m) * p.ldc + n) = v;
+                }
+                asm volatile("" ::: "memory");
+            };
+            out(C, silu);
+            if (Z) out(Z, false);
+            return;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < FB; ++j)
 #pragma unroll
@@ -335,7 +455,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                 if (m >= left_m) continue;
                 if (PROD == PROD_WEIGHT && part) {
                     float* const to = part + (long)(m0 + m) * N + n;
-                    if (p.quads) *reinterpret_cast<f32x4*>(to) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                    if (p.pieces >= 4) *reinterpret_cast<f32x4*>(to) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
                     else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) if (r < left_n) to[r] = acc[i][j][4 * g + r];
@@ -347,10 +467,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                 for (int r = 0; r < 4; ++r) {
                     const float v = acc[i][j][4 * g + r] + bv[r];
                     z[r] = (T)v;
-                    y[r] = silu ? (T)silu_value(v) : (T)v;
+                    y[r] = silu ? (T)silu_value<T>(v) : (T)v;
                 }
                 const long at = (long)m * p.ldc + n;
-                if (p.quads) {
+                if (p.pieces >= 4) {
                     *reinterpret_cast<V4*>(C + at) = y;
                     if (Z) *reinterpret_cast<V4*>(Z + at) = z;
                 } else {
@@ -420,7 +540,7 @@ __global__ __launch_bounds__(256) void k_silu_back(const int* __restrict__ activ
         VT o;
         T* oe = reinterpret_cast<T*>(&o);
 #pragma unroll
-        for (int j = 0; j < V; ++j) oe[j] = (T)((float)ge[j] * silu_slope((float)ze[j]));
+        for (int j = 0; j < V; ++j) oe[j] = (T)((float)ge[j] * silu_slope<T>((float)ze[j]));
         *reinterpret_cast<VT*>(dz + i * V) = o;
     }
 }
@@ -433,7 +553,7 @@ int launch_tiles(const ProdArgs& p, hipStream_t s) {
     if (blocks > 0x003fffffL) return fail("expert_linear: %ld tiles are more than a launch holds", blocks);
     if (blocks) hipLaunchKernelGGL((k_product<T, PROD, TM, TN, WM, WN, NST>), dim3((unsigned)blocks), dim3(64 * WM * WN), NST * (TM + TN) * 128, s, p, (int)tm, (int)tn);
     if (cut) {
-        const bool four = p.quads && p.M % 4 == 0;
+        const bool four = p.pieces >= 4 && p.M % 4 == 0;
         const long per = cdiv((long)p.M * p.N + p.M, four ? 1024 : 256);
         const dim3 grid((unsigned)(per < 1024 ? per : 1024), p.E);
         if (four) hipLaunchKernelGGL((k_join_parts<T, 4>), grid, dim3(256), 0, s, p);
@@ -504,7 +624,10 @@ struct Operand {
     }
 };
 template <typename T>
-bool quads_ok(long N, long ldc, const void* c, const void* z) { return N % 4 == 0 && ldc % 4 == 0 && (((uintptr_t)c | (uintptr_t)z) & (4 * sizeof(T) - 1)) == 0; }
+int result_pieces(long N, long ldc, const void* c, const void* z, const void* bias) {
+    const int b = common_align({(uint64_t)N * sizeof(T), (uint64_t)ldc * sizeof(T), (uint64_t)(uintptr_t)c, (uint64_t)(uintptr_t)z, (uint64_t)(uintptr_t)bias}) / (int)sizeof(T);
+    return b >= 8 ? 8 : (b >= 4 ? 4 : 1);
+}
 
 // the operands of a product, as the entry points name them
 template <typename T>
@@ -541,6 +664,6 @@ int run_product(ProdArgs p, int64_t inp, int64_t out, const void* a, int64_t a_s
     ob.place(&p.b, &p.ldb, &ws, s);
     p.b_expert = (PROD == PROD_WEIGHT ? 0 : out) * p.ldb;
     p.parts = reinterpret_cast<float*>(ws);
-    p.quads = quads_ok<T>(p.N, p.ldc, p.c, p.z);
+    p.pieces = result_pieces<T>(p.N, p.ldc, p.c, p.z, p.bias);
     return launch_prod<T, PROD>(p, s);
 }
