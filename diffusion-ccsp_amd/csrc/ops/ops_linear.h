@@ -68,21 +68,6 @@ template <typename T> __device__ __forceinline__ float sigmoid_of(float z) {
 template <typename T> __device__ __forceinline__ float silu_value(float z) { return sizeof(T) == 4 ? z / (1.0f + expf(-z)) : z * sigmoid_of<T>(z); }
 template <typename T> __device__ __forceinline__ float silu_slope(float z) { const float s = sigmoid_of<T>(z); return s * (1.0f + z * (1.0f - s)); }
 
-// s + the eight values of v, in 32 bits
-__device__ __forceinline__ float add_all(__attribute__((ext_vector_type(8))) bf16 v, float s) {
-    typedef bf16 V2 __attribute__((ext_vector_type(2)));
-    const V2 one = {(bf16)1.0f, (bf16)1.0f};
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(V2{v[i], v[i + 1]}, one, s, false);
-    return s;
-}
-__device__ __forceinline__ float add_all(__attribute__((ext_vector_type(8))) fp16 v, float s) {
-    typedef fp16 V2 __attribute__((ext_vector_type(2)));
-    const V2 one = {(fp16)1.0f, (fp16)1.0f};
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(V2{v[i], v[i + 1]}, one, s, false);
-    return s;
-}
 template <typename T> struct Vec8 { typedef T t __attribute__((ext_vector_type(8))); };
 __device__ __forceinline__ f32x4 mfma16(Vec8<bf16>::t a, Vec8<bf16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma16(Vec8<fp16>::t a, Vec8<fp16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -265,9 +250,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     const T* A = static_cast<const T*>(p.a) + (PROD == PROD_WEIGHT ? (long)r0 * p.lda + m0 : (long)r0 * p.lda);
     const T* B = static_cast<const T*>(p.b) + (PROD == PROD_WEIGHT ? (long)r0 * p.ldb + n0 : e * p.b_expert + (BKC ? (long)n0 * p.ldb : (long)n0));
     Acc acc[FA][FB] = {};
-    // the bias gradient (sum over k of A) is made on the way by the waves that hold the first columns of n: vector additions beside the matrix
-    // instructions, each lane over the k that it holds
-    const bool sums = PROD == PROD_WEIGHT && p.sum && n0 + wn == 0;
+    // The bias gradient (sum over k of A) is made on the way, by the blocks of the first columns.  32 bits: one addition beside each matrix instruction, by the
+    // waves that hold the first columns, over the k that a lane holds.  16 bits: the waves share a stage's k rows, a lane adds up four columns of
+    // its rows from LDS; as a product with ones it cost these blocks an eighth of their time and a second set of fragments.
+    const bool sums = PROD == PROD_WEIGHT && p.sum && n0 + (F32 ? wn : 0) == 0;
+    constexpr int LPR = TM / 4, RPI = 64 / LPR, WAVES = WM * WN;             // lanes of a k row, k rows of an access
+    float col[4] = {};
     float sum[FA] = {};
     // 32 bits: a chain of K additions into one register would lose sqrt(K) roundings' worth; every FLUSH stages it goes into a second one
     constexpr int FLUSH = 4;
@@ -320,40 +308,39 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                         }
                         if constexpr (F32) { if (S) sum[i] += fa[set][i][k]; }
                     }
-                if constexpr (!F32) if (S) {
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int i = 0; i < FA; ++i) sum[i] = add_all(fa[set][i], sum[i]);
-                }
             };
             if (NST <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            // (the sums' registers and a second set of fragments do not fit beside a 128 x 64 part: there a step waits for its own fragments)
-            constexpr bool AHEAD = !(S && TM == 256);
-            if (AHEAD) read(0, 0, 0);
+            read(0, 0, 0);
             int buf = 0;
             for (int st = 0; st < stages; ++st) {
+                if constexpr (!F32 && PROD == PROD_WEIGHT) if (sums) {
+#pragma unroll
+                    for (int i = 0; i < SK / WAVES / RPI; ++i) {
+                        const int k = wave * (SK / WAVES) + i * RPI + lane / LPR, l = lane % LPR;
+                        const typename VecOf<T, 4>::type v = *reinterpret_cast<const typename VecOf<T, 4>::type*>(sm + buf * STAGE + k * TM + (((l >> 2) ^ block_swizzle<TM>(k)) << 4) + 4 * (l & 3));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) col[r] += (float)v[r];
+                    }
+                }
 #pragma unroll
                 for (int ks = 0; ks < KS - 1; ++ks) {
-                    if (AHEAD) read((ks + 1) & 1, buf, ks + 1); else read(0, buf, ks);
-                    multiply(AHEAD ? ks & 1 : 0);
-                    if (AHEAD) spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
+                    read((ks + 1) & 1, buf, ks + 1);
+                    multiply(ks & 1);
+                    spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
                 }
-                if (!AHEAD) { read(0, buf, KS - 1); multiply(0); }
                 if (st + NST - 1 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * L) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
                 if (st + NST < stages) fetch(st + NST, buf);
                 buf = buf + 1 == NST ? 0 : buf + 1;
-                if (AHEAD) {
-                    read(0, buf, 0);                             // (behind the last stage: whatever lies there, unused)
-                    asm volatile("" ::: "memory");               // (or the compiler reads them in the next round after all)
-                    multiply((KS - 1) & 1);
-                    spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
-                }
+                read(0, buf, 0);                                 // (behind the last stage: whatever lies there, unused)
+                asm volatile("" ::: "memory");                   // (or the compiler reads them in the next round after all)
+                multiply((KS - 1) & 1);
+                spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
                 if constexpr (F32) {
                     if ((st + 1) % FLUSH == 0) {
                         asm volatile("" ::: "memory");          // (a branch, not 48 selects every stage)
@@ -367,7 +354,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                 }
             }
         };
-        if (PROD == PROD_WEIGHT && sums) loop(std::true_type{}); else loop(std::false_type{});
+        if (F32 && PROD == PROD_WEIGHT && sums) loop(std::true_type{}); else loop(std::false_type{});
     }
     if constexpr (F32) {
 #pragma unroll
@@ -382,15 +369,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     T* Z = PROD == PROD_FORWARD && p.z ? static_cast<T*>(p.z) + (long)r0 * p.ldc : nullptr;
     const T* bias = PROD == PROD_FORWARD && p.bias && e < p.E ? static_cast<const T*>(p.bias) + (long)e * N : nullptr;
     const bool silu = PROD == PROD_FORWARD && p.silu && e < p.E;
-    if (sums) {
+    if (PROD == PROD_WEIGHT && sums) {
+        auto put = [&](int m, float v) {
+            if (m >= left_m) return;
+            if (part) part[(long)p.M * p.N + m0 + m] = v; else static_cast<T*>(p.sum)[(long)e * p.M + m0 + m] = (T)v;
+        };
+        if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < FA; ++i) {
-            float v = sum[i] + __shfl_xor(sum[i], 32);           // (the lanes of a row hold its k between them)
-            if (!F32) v += __shfl_xor(v, 16);
-            const int m = wm + G * i + lane;
-            if (lane < G && m < left_m) {
-                if (part) part[(long)p.M * p.N + m0 + m] = v; else static_cast<T*>(p.sum)[(long)e * p.M + m0 + m] = (T)v;
+            for (int i = 0; i < FA; ++i) {
+                const float v = sum[i] + __shfl_xor(sum[i], 32);       // (two lanes hold a row's k between them)
+                if (lane < G) put(wm + G * i + lane, v);
             }
+        } else {
+            // [WAVES][TM] sums in LDS, added in order (the whole block is here: `sums` is the block's; LDS is free since the last barrier)
+            float* const cs = reinterpret_cast<float*>(lds);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                for (int o = LPR; o < 64; o <<= 1) col[r] += __shfl_xor(col[r], o);
+                if (lane < LPR) cs[wave * TM + 4 * lane + r] = col[r];
+            }
+            __syncthreads();
+            if (threadIdx.x < TM) {
+                float v = 0.0f;
+                for (int w = 0; w < WAVES; ++w) v += cs[w * TM + threadIdx.x];
+                put(threadIdx.x, v);
+            }
+            __syncthreads();                                     // (the results go through the same LDS)
         }
     }
     if (PROD == PROD_WEIGHT && !p.c) return;                     // (the sums alone)
@@ -563,15 +567,19 @@ int launch_tiles(const ProdArgs& p, hipStream_t s) {
     return 0;
 }
 
-// Tiles of a product by how many there are: 256 x 256 where they go round the CUs a few times, 128 x 128, and 64 x 64 with four stages where even
-// those are too few to keep enough bytes on their way (one token's experts, short prompts).  A weight gradient over few rows an expert writes more than it
-// multiplies: there two blocks a CU write while another multiplies (32 experts of 256 rows, 2048 x 1408: 110 us by 128, 128 us by 256).
+// Tiles of a product by how many there are: 256 x 256 where they fill the CUs, 128 x 128, and 64 x 64 with four stages where even those are too few to
+// keep enough bytes on their way (one token's experts, short prompts).  Measured in bf16, 128 against 256:
+//   rows x outputs: 8192 rows, 1 expert, 4096 -> 4096 (528 tiles of 256): 282 us against 244; 20264 rows, 13 experts, 2048 -> 2048 (736): 181 against 166;
+//   but 16384 rows, 16 experts, 2048 -> 2048 (640): 150 against 162: at 1024 rows an expert an eighth of the 256-row tiles is empty
+//   weight gradient: 8192 rows, 1 expert, 4096 x 4096 (256 tiles): 260 against 228; 32768 rows, 8 experts, 2048 x 1024 (256): 188 against 128; but 32 experts of
+//   256 rows, 2048 x 1408: 110 against 128: few rows an expert write more than they multiply, and a CU's two small blocks do one while the other does the other
 inline long prod_tiles(bool weight, long R, long E, long M, long N, int l) { return (weight ? E * cdiv(M, 1l << l) : most_tiles(R, E, l)) * cdiv(N, 1l << l); }
 enum { TILE_64 = 6, TILE_128 = 7, TILE_256 = 8 };
 template <typename T>
 int prod_tile(bool weight, long R, long E, long M, long N) {
     if (sizeof(T) == 4) return TILE_64;
-    if (prod_tiles(weight, R, E, M, N, 8) >= 1024 && (!weight || R >= 1024 * E)) return TILE_256;
+    const long big = prod_tiles(weight, R, E, M, N, 8);
+    if (weight ? big >= 256 && R >= 1024 * E : big >= 1024 || (big >= 512 && R >= 1280 * E)) return TILE_256;
     return prod_tiles(weight, R, E, M, N, 7) >= 512 ? TILE_128 : TILE_64;
 }
 
