@@ -84,10 +84,10 @@ def lib():
     _check_version(OPS_SO, int(L.ccsp_ops_version()))
     L.ccsp_ops_route_workspace.argtypes = [i64, i32, i64, i32]
     L.ccsp_ops_route_workspace.restype = i64
-    L.ccsp_ops_route.argtypes = [vp, vp, i32, i64, i32, i32, i64] + [vp] * 7 + [i64, vp]
-    L.ccsp_ops_rows_gather.argtypes = [i32, i64, i64, vp, i64, vp, vp, vp]
+    L.ccsp_ops_route.argtypes = [vp, vp, i32, i64, i32, i32, i64] + [vp] * 8 + [i64, vp]
+    L.ccsp_ops_rows_gather.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6
     L.ccsp_ops_rows_combine.argtypes = [i32, i64, i64, i32, vp, vp, vp, vp, i32, vp, i64, vp, vp]
-    L.ccsp_ops_rows_back.argtypes = [i32, i64, i64, vp, vp, vp, i32, vp, i64, vp, i64, vp, vp, vp]
+    L.ccsp_ops_rows_back.argtypes = [i32, i64, i64] + [vp] * 5 + [i32, vp, i64, vp, i64, vp, vp, vp]
     L.ccsp_ops_linear_workspace.argtypes = [i32, i32, i32, i64, i64, i64, vp, i64, vp, i64]
     L.ccsp_ops_linear_workspace.restype = i64
     L.ccsp_ops_linear.argtypes = [i32, i32, i64, i64, i64, vp, vp, i64, vp, vp, i32, vp, vp, vp, i64, vp]

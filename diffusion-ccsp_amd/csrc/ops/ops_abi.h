@@ -11,19 +11,19 @@ int64_t ccsp_ops_route_workspace(int64_t n_assign, int32_t n_experts, int64_t n_
 }
 
 int ccsp_ops_route(const void* expert, const void* token, int32_t id_bits, int64_t n_assign, int32_t k, int32_t n_experts, int64_t n_tokens, int32_t* offsets, int32_t* rows, int32_t* assign,
-                   int32_t* row_token, int32_t* token_ptr, int32_t* token_assign, void* workspace, int64_t workspace_bytes, void* stream) {
+                   int32_t* row_token, int32_t* place, int32_t* token_ptr, int32_t* token_assign, void* workspace, int64_t workspace_bytes, void* stream) {
     CCSP_OPS_CHECK(id_bits == 32 || id_bits == 64, "route: ids of 32 or 64 bits, not %d", id_bits);
     CCSP_OPS_CHECK(n_assign >= 0 && n_assign <= CCSP_OPS_MAX_ASSIGN, "route: %lld assignments out of range", (long long)n_assign);
     CCSP_OPS_CHECK(n_tokens >= 0 && n_tokens <= CCSP_OPS_MAX_ASSIGN, "route: %lld tokens out of range", (long long)n_tokens);
     CCSP_OPS_CHECK(n_experts >= 1 && n_experts <= CCSP_OPS_MAX_EXPERTS, "route: %d experts, supported are 1 to %d", n_experts, CCSP_OPS_MAX_EXPERTS);
     const bool list = token_ptr != nullptr;                      // (an empty list may have no address)
     CCSP_OPS_CHECK(list || (!token && k >= 1 && n_assign == n_tokens * k), "route: %lld assignments are not %lld tokens of %d each (list tokens need token_ptr)", (long long)n_assign, (long long)n_tokens, k);
-    CCSP_OPS_CHECK(offsets && (n_assign == 0 || (expert && rows && assign && row_token)), "route: null argument");
+    CCSP_OPS_CHECK(offsets && (n_assign == 0 || (expert && rows && assign && row_token && place)), "route: null argument");
     CCSP_OPS_CHECK(!list || n_assign == 0 || (token && token_assign), "route: list tokens need token, token_ptr and token_assign");
     CCSP_OPS_CHECK(workspace_bytes >= ccsp_ops_route_workspace(n_assign, n_experts, n_tokens, list) && (workspace || workspace_bytes == 0), "route: workspace of %lld bytes is too small",
                    (long long)workspace_bytes);
     const RouteIds r = {expert, token, id_bits == 64, (int)n_assign, k, n_experts, (int)n_tokens};
-    const RouteOut o = {offsets, rows, assign, row_token, token_ptr, token_assign};
+    const RouteOut o = {offsets, rows, assign, row_token, place, token_ptr, token_assign};
     return route(r, o, static_cast<int*>(workspace), (hipStream_t)stream);
 }
 
@@ -33,12 +33,13 @@ static int check_rows(const char* who, int32_t type, int64_t n, int64_t width) {
     return 0;
 }
 
-int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void* src, int64_t src_stride, const int32_t* row_token, void* dst, void* stream) {
+int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void* src, int64_t src_stride, const int32_t* row_token, const int32_t* assign, const int32_t* place,
+                         const int32_t* token_assign, void* dst, void* stream) {
     if (check_rows("rows_gather", type, n_rows, width)) return 1;
     if (n_rows == 0 || width == 0) return 0;
-    CCSP_OPS_CHECK(row_token && dst, "rows_gather: null argument");
+    CCSP_OPS_CHECK(row_token && assign && place && dst, "rows_gather: null argument");
     const long b = type_bytes(type);
-    return rows_gather(n_rows, width * b, src, src_stride * b, row_token, dst, width * b, (hipStream_t)stream);
+    return rows_gather({row_token, assign, place, token_assign}, n_rows, width * b, src, src_stride * b, dst, width * b, (hipStream_t)stream);
 }
 
 int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
@@ -53,15 +54,15 @@ int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t
     });
 }
 
-int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_t* assign, const int32_t* row_token, const void* weight, int32_t weight_type, const void* dy, int64_t dy_stride,
+int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_t* row_token, const int32_t* assign, const int32_t* place, const int32_t* token_assign, const void* weight, int32_t weight_type, const void* dy, int64_t dy_stride,
                        const void* src, int64_t src_stride, void* d_src, void* d_weight, void* stream) {
     if (check_rows("rows_back", type, n_rows, width)) return 1;
     if (n_rows == 0) return 0;
-    CCSP_OPS_CHECK(assign && row_token && (width == 0 || (d_src || d_weight)), "rows_back: null argument");
+    CCSP_OPS_CHECK(assign && row_token && place && (width == 0 || (d_src || d_weight)), "rows_back: null argument");
     CCSP_OPS_CHECK((!weight && !d_weight) || weight_type == CCSP_OPS_F32 || weight_type == type, "rows_back: weights are 32 bits or of the rows' type");
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return rows_back<T>(n_rows, (int)width, assign, row_token, weight, weight_type == CCSP_OPS_F32, (const T*)dy, dy_stride, (const T*)src, src_stride, (T*)d_src, d_src ? width : 0, d_weight,
+        return rows_back<T>({row_token, assign, place, token_assign}, n_rows, (int)width, weight, weight_type == CCSP_OPS_F32, (const T*)dy, dy_stride, (const T*)src, src_stride, (T*)d_src, d_src ? width : 0, d_weight,
                             (hipStream_t)stream);
     });
 }
@@ -140,7 +141,9 @@ int ccsp_ops_linear_back_weight(int32_t type, int32_t n_experts, int64_t n_rows,
 int64_t ccsp_ops_norm_workspace(int32_t n_tensors, const int64_t* sizes) {
     if (n_tensors < 0 || (n_tensors && !sizes)) return -1;
     int64_t b = 1;
-    for (int32_t i = 0; i < n_tensors; ++i) { if (sizes[i] < 0) return -1; b += cdiv(sizes[i], NORM_CHUNK); }
+    for (int32_t i = 0; i < n_tensors; ++i) if (sizes[i] < 0) return -1;
+    const long chunk = norm_chunk_for(n_tensors, sizes);
+    for (int32_t i = 0; i < n_tensors; ++i) b += cdiv(sizes[i], chunk);
     return 8 * b;
 }
 

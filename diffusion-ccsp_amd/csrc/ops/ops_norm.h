@@ -9,7 +9,14 @@
 // The tensor table travels in the kernel arguments, NORM_TENSORS a launch: no copy to the device, nothing that a captured graph
 // would have to find again at replay but the addresses themselves.
 constexpr int NORM_TENSORS = 112;
-constexpr int NORM_CHUNK = 16384;                                // elements of a block
+// Elements of a block.  Few elements are cut finer, so that there are blocks for every CU and short chains (300 odd tensors of 400000 elements in all: clip 8.0 -> 5.1 us a launch);
+// many are not, because each block ends with a sum over its threads.
+constexpr long NORM_FINE = 4096, NORM_COARSE = 16384, NORM_MANY = 1l << 26;
+inline long norm_chunk_for(int count, const int64_t* n) {
+    long total = 0;
+    for (int i = 0; i < count; ++i) total += n[i];
+    return total < NORM_MANY ? NORM_FINE : NORM_COARSE;
+}
 
 struct NormTable {
     const void* in[NORM_TENSORS];
@@ -17,7 +24,7 @@ struct NormTable {
     long n[NORM_TENSORS];
     int first[NORM_TENSORS + 1];                                 // first block of a tensor
     unsigned char type[NORM_TENSORS];
-    int count;
+    int count, chunk;
 };
 
 // the tensor of block b: the number of first blocks <= b, less one (tensors without elements share their first block with the next)
@@ -68,8 +75,8 @@ __device__ __forceinline__ double block_sum(double s, double* part, int waves) {
 __global__ __launch_bounds__(256) void k_norm_part(NormTable t, double* part) {
     __shared__ double sums[4];
     const int i = norm_tensor(t, blockIdx.x);
-    const long at = (long)(blockIdx.x - t.first[i]) * NORM_CHUNK;
-    const long n = t.n[i] - at < NORM_CHUNK ? t.n[i] - at : NORM_CHUNK;
+    const long at = (long)(blockIdx.x - t.first[i]) * t.chunk;
+    const long n = t.n[i] - at < t.chunk ? t.n[i] - at : t.chunk;
     double s;
     if (t.type[i] == CCSP_OPS_F32) s = norm_chunk(static_cast<const float*>(t.in[i]) + at, n);
     else if (t.type[i] == CCSP_OPS_BF16) s = norm_chunk(static_cast<const bf16*>(t.in[i]) + at, n);
@@ -142,8 +149,8 @@ __global__ __launch_bounds__(256) void k_norm_clip(NormTable t, int blocks, cons
     const int b = blocks - 1 - blockIdx.x;                       // from the end: what the norm read last is still in the last-level cache
     const int i = norm_tensor(t, b);
     if (c == 1.0f && t.in[i] == t.out[i]) return;                // g x 1 in place
-    const long at = (long)(b - t.first[i]) * NORM_CHUNK;
-    const long n = t.n[i] - at < NORM_CHUNK ? t.n[i] - at : NORM_CHUNK;
+    const long at = (long)(b - t.first[i]) * t.chunk;
+    const long n = t.n[i] - at < t.chunk ? t.n[i] - at : t.chunk;
     if (t.type[i] == CCSP_OPS_F32) clip_chunk(static_cast<const float*>(t.in[i]) + at, static_cast<float*>(t.out[i]) + at, n, c);
     else if (t.type[i] == CCSP_OPS_BF16) clip_chunk(static_cast<const bf16*>(t.in[i]) + at, static_cast<bf16*>(t.out[i]) + at, n, c);
     else clip_chunk(static_cast<const fp16*>(t.in[i]) + at, static_cast<fp16*>(t.out[i]) + at, n, c);
@@ -152,14 +159,16 @@ __global__ __launch_bounds__(256) void k_norm_clip(NormTable t, int blocks, cons
 // hands tables of at most NORM_TENSORS tensors that have elements to f(table, blocks, blocks before it), first to last or last to first
 template <typename F>
 int norm_tables(int count, const void* const* in, void* const* out, const int64_t* n, const int32_t* type, F&& f) {
+    const long chunk = norm_chunk_for(count, n);
     long before = 0;
     for (int i = 0; i < count;) {
         NormTable t;
         int blocks = 0;
         t.count = 0;
+        t.chunk = (int)chunk;
         for (; i < count && t.count < NORM_TENSORS; ++i) {
             if (n[i] == 0) continue;
-            const long b = cdiv(n[i], NORM_CHUNK);
+            const long b = cdiv(n[i], chunk);
             if (b > 0x800000L) return fail("tensor %d has too many elements", i);
             if (t.count && blocks + b > 0x800000L) break;      // (a grid holds 2^32 threads)
             t.in[t.count] = in[i]; t.out[t.count] = out ? out[i] : nullptr; t.n[t.count] = n[i]; t.type[t.count] = (unsigned char)type[i];

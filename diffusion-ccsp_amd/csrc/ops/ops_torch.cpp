@@ -51,20 +51,21 @@ struct Plan {
     int64_t n_experts = 0, n_tokens = 0, n_rows = 0, k = 0;
     bool listed = false;
     std::vector<int64_t> shape;
-    int64_t at(int which) const {                                // first element of: offsets, rows, assign, row_token, token_ptr, token_assign, the end
-        const int64_t o[7] = {0, n_experts + 1, n_experts + 1 + n_rows, n_experts + 1 + 2 * n_rows, n_experts + 1 + 3 * n_rows, n_experts + 2 + 3 * n_rows + n_tokens,
-                              n_experts + 2 + 4 * n_rows + n_tokens};
-        return which == 6 && !listed ? o[4] : o[which];
+    enum { OFFSETS, ROWS, ASSIGN, ROW_TOKEN, PLACE, TOKEN_PTR, TOKEN_ASSIGN, END };
+    int64_t at(int which) const {                                // first element of a part
+        const int64_t a = n_experts + 1, o[8] = {0, a, a + n_rows, a + 2 * n_rows, a + 3 * n_rows, a + 4 * n_rows, a + 4 * n_rows + n_tokens + 1, a + 5 * n_rows + n_tokens + 1};
+        return which == END && !listed ? o[TOKEN_PTR] : o[which];
     }
     int32_t* p(int which) const { return buf.data_ptr<int32_t>() + at(which); }
     Tensor view(int which, int64_t n) const { return buf.narrow(0, at(which), n); }
-    Tensor offsets() const { return view(0, n_experts + 1); }
-    Tensor rows() const { return view(1, n_rows); }
-    Tensor assign() const { return view(2, n_rows); }
-    Tensor row_token() const { return view(3, n_rows); }
-    MaybeTensor token_ptr() const { return listed ? MaybeTensor(view(4, n_tokens + 1)) : MaybeTensor(); }
-    MaybeTensor token_assign() const { return listed ? MaybeTensor(view(5, n_rows)) : MaybeTensor(); }
-    Tensor counts() const { return view(1 - 1, n_experts + 1).diff(); }
+    int32_t* token_order() const { return listed ? p(TOKEN_ASSIGN) : nullptr; }
+    Tensor offsets() const { return view(OFFSETS, n_experts + 1); }
+    Tensor rows() const { return view(ROWS, n_rows); }
+    Tensor assign() const { return view(ASSIGN, n_rows); }
+    Tensor row_token() const { return view(ROW_TOKEN, n_rows); }
+    MaybeTensor token_ptr() const { return listed ? MaybeTensor(view(TOKEN_PTR, n_tokens + 1)) : MaybeTensor(); }
+    MaybeTensor token_assign() const { return listed ? MaybeTensor(view(TOKEN_ASSIGN, n_rows)) : MaybeTensor(); }
+    Tensor counts() const { return offsets().diff(); }
     // what an autograd node keeps of a plan
     void save(AutogradContext* c) const { c->saved_data["plan"] = std::vector<int64_t>{n_experts, n_tokens, n_rows, k, listed}; }
     static Plan load(AutogradContext* c, const Tensor& buf) {
@@ -104,24 +105,24 @@ std::shared_ptr<Plan> route(const Tensor& expert_in, int64_t n_experts, const Ma
     const int64_t need = ccsp_ops_route_workspace(q->n_rows, (int32_t)n_experts, q->n_tokens, q->listed);
     VALUE(need >= 0, "route: ", q->n_rows, " assignments of ", q->n_tokens, " tokens are out of range");
     On on(expert);
-    q->buf = at::empty({q->at(6)}, expert.options().dtype(at::kInt));
+    q->buf = at::empty({q->at(Plan::END)}, expert.options().dtype(at::kInt));
     const Tensor ws = at::empty({need}, expert.options().dtype(at::kByte));
-    run(ccsp_ops_route(ptr(expert), ptr(tokens), (int32_t)expert.element_size() * 8, q->n_rows, (int32_t)q->k, (int32_t)n_experts, q->n_tokens, q->p(0), q->p(1), q->p(2), q->p(3),
-                       q->listed ? q->p(4) : nullptr, q->listed ? q->p(5) : nullptr, ptr(ws), need, on.stream));
+    run(ccsp_ops_route(ptr(expert), ptr(tokens), (int32_t)expert.element_size() * 8, q->n_rows, (int32_t)q->k, (int32_t)n_experts, q->n_tokens, q->p(Plan::OFFSETS), q->p(Plan::ROWS),
+                       q->p(Plan::ASSIGN), q->p(Plan::ROW_TOKEN), q->p(Plan::PLACE), q->listed ? q->p(Plan::TOKEN_PTR) : nullptr, q->token_order(), ptr(ws), need, on.stream));
     return q;
 }
 
 Tensor gather(const Tensor& src_in, const Plan& q) {
     On on(src_in);
     const Tensor src = rows_of(src_in), out = at::empty({q.n_rows, src.size(1)}, src.options());
-    run(ccsp_ops_rows_gather(code(src), q.n_rows, src.size(1), ptr(src), src.stride(0), q.p(3), ptr(out), on.stream));
+    run(ccsp_ops_rows_gather(code(src), q.n_rows, src.size(1), ptr(src), src.stride(0), q.p(Plan::ROW_TOKEN), q.p(Plan::ASSIGN), q.p(Plan::PLACE), q.token_order(), ptr(out), on.stream));
     return out;
 }
 
 Tensor combine(const Tensor& src_in, const Plan& q, const Tensor& weights) {
     On on(src_in);
     const Tensor src = rows_of(src_in), out = at::empty({q.n_tokens, src.size(1)}, src.options());
-    run(ccsp_ops_rows_combine(code(src), q.n_tokens, src.size(1), (int32_t)q.k, q.listed ? q.p(4) : nullptr, q.listed ? q.p(5) : nullptr, q.p(1), ptr(weights),
+    run(ccsp_ops_rows_combine(code(src), q.n_tokens, src.size(1), (int32_t)q.k, q.listed ? q.p(Plan::TOKEN_PTR) : nullptr, q.token_order(), q.p(Plan::ROWS), ptr(weights),
                               weights.defined() ? code(weights) : CCSP_OPS_F32, ptr(src), src.stride(0), ptr(out), on.stream));
     return out;
 }
@@ -169,7 +170,7 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
         const Tensor g = rows_of(grads[0]), ys = want_w ? rows_of(saved[1]) : Tensor();
         On on(g);
         const Tensor d_ys = want_ys ? at::empty({q.n_rows, g.size(1)}, g.options()) : Tensor(), d_w = want_w ? at::empty(weights.sizes(), weights.options()) : Tensor();
-        run(ccsp_ops_rows_back(code(g), q.n_rows, g.size(1), q.p(2), q.p(3), ptr(weights), code(weights), ptr(g), g.stride(0), ptr(ys), want_w ? ys.stride(0) : 0, ptr(d_ys), ptr(d_w),
+        run(ccsp_ops_rows_back(code(g), q.n_rows, g.size(1), q.p(Plan::ROW_TOKEN), q.p(Plan::ASSIGN), q.p(Plan::PLACE), q.token_order(), ptr(weights), code(weights), ptr(g), g.stride(0), ptr(ys), want_w ? ys.stride(0) : 0, ptr(d_ys), ptr(d_w),
                                on.stream));
         return first_order("combine_rows", more, {d_ys, d_w, Tensor(), Tensor()});
     }
@@ -223,7 +224,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const Tensor& bias,
     const Tensor y = at::empty({q.n_rows, O}, x.options());
     if (z) *z = at::empty({q.n_rows, O}, x.options());
     const Space ws(CCSP_OPS_FORWARD, x, weight, q, O, I);
-    run(ccsp_ops_linear(code(x), (int32_t)q.n_experts, q.n_rows, I, O, q.p(0), ptr(x), x.stride(0), ptr(weight), ptr(bias), (int32_t)act, ptr(y), z ? ptr(*z) : nullptr, ptr(ws.t), ws.bytes,
+    run(ccsp_ops_linear(code(x), (int32_t)q.n_experts, q.n_rows, I, O, q.p(Plan::OFFSETS), ptr(x), x.stride(0), ptr(weight), ptr(bias), (int32_t)act, ptr(y), z ? ptr(*z) : nullptr, ptr(ws.t), ws.bytes,
                         on.stream));
     return y;
 }
@@ -253,19 +254,19 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
         if (c->saved_data["act"].toInt()) {
             const Tensor g = dz;
             dz = at::empty({q.n_rows, O}, g.options());
-            run(ccsp_ops_linear_silu_back(type, E, q.n_rows, O, q.p(0), ptr(g), g.stride(0), ptr(z), ptr(dz), on.stream));
+            run(ccsp_ops_linear_silu_back(type, E, q.n_rows, O, q.p(Plan::OFFSETS), ptr(g), g.stride(0), ptr(z), ptr(dz), on.stream));
         }
         if (c->needs_input_grad(0)) {
             d_x = at::empty({q.n_rows, I}, dz.options());
             const Space ws(CCSP_OPS_BACK_INPUT, dz, weight, q, O, I);
-            run(ccsp_ops_linear_back_input(type, E, q.n_rows, I, O, q.p(0), ptr(dz), dz.stride(0), ptr(weight), ptr(d_x), ptr(ws.t), ws.bytes, on.stream));
+            run(ccsp_ops_linear_back_input(type, E, q.n_rows, I, O, q.p(Plan::OFFSETS), ptr(dz), dz.stride(0), ptr(weight), ptr(d_x), ptr(ws.t), ws.bytes, on.stream));
         }
         const bool want_w = c->needs_input_grad(1), want_b = c->needs_input_grad(2);
         if (want_w || want_b) {
             if (want_w) d_w = at::empty({E, O, I}, dz.options());
             if (want_b) d_b = at::empty({E, O}, dz.options());
             const Space ws(CCSP_OPS_BACK_WEIGHT, dz, x, q, O, I);
-            run(ccsp_ops_linear_back_weight(type, E, q.n_rows, I, O, q.p(0), ptr(dz), dz.stride(0), ptr(x), x.stride(0), ptr(d_w), ptr(d_b), ptr(ws.t), ws.bytes, on.stream));
+            run(ccsp_ops_linear_back_weight(type, E, q.n_rows, I, O, q.p(Plan::OFFSETS), ptr(dz), dz.stride(0), ptr(x), x.stride(0), ptr(d_w), ptr(d_b), ptr(ws.t), ws.bytes, on.stream));
         }
         return first_order("expert_linear", more, {d_x, d_w, d_b, Tensor(), Tensor(), Tensor()});
     }

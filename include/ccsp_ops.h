@@ -43,15 +43,19 @@ const char* ccsp_ops_last_error(void);
  *   rows         [n_assign]       row of every assignment (by expert, then by assignment), -1 if dropped
  *   assign       [n_assign]       assignment of every row; behind the last active row ~a of the dropped ones
  *   row_token    [n_assign]       token of every row, -1 behind the last active row
- *   token_ptr    [n_tokens + 1], token_assign [n_assign] (both or neither: token_ptr says that there is a list): the active assignments of every token, ascending
+ *   place        [n_assign]       the inverse of assign: row p of every assignment, ~p if dropped
+ *   token_ptr    [n_tokens + 1], token_assign [n_assign] (both or neither: token_ptr says that there is a list): the active assignments of every token, ascending;
+ *                                 the dropped ones behind them
  * workspace: ccsp_ops_route_workspace bytes (-1: an argument is out of range), free again when the call's work is done. */
 int64_t ccsp_ops_route_workspace(int64_t n_assign, int32_t n_experts, int64_t n_tokens, int32_t list_tokens);
 int ccsp_ops_route(const void* expert, const void* token, int32_t id_bits, int64_t n_assign, int32_t k, int32_t n_experts, int64_t n_tokens,
-                   int32_t* offsets, int32_t* rows, int32_t* assign, int32_t* row_token, int32_t* token_ptr, int32_t* token_assign,
+                   int32_t* offsets, int32_t* rows, int32_t* assign, int32_t* row_token, int32_t* place, int32_t* token_ptr, int32_t* token_assign,
                    void* workspace, int64_t workspace_bytes, void* stream);
 
-/* dst[p] = src[row_token[p]] for p < n_rows, zeros where row_token[p] < 0.  dst [n_rows, width] contiguous. */
-int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void* src, int64_t src_stride, const int32_t* row_token, void* dst, void* stream);
+/* dst[p] = src[row_token[p]] for p < n_rows, zeros where row_token[p] < 0.  dst [n_rows, width] contiguous.  row_token, assign, place, token_assign (NULL without
+ * listed tokens): the plan's. */
+int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void* src, int64_t src_stride, const int32_t* row_token, const int32_t* assign, const int32_t* place,
+                         const int32_t* token_assign, void* dst, void* stream);
 /* dst[n] = sum over the token's active assignments a, ascending, of weight[a] * src[rows[a]]; sums in 32 bits, rounded once.  token_ptr /
  * token_assign NULL: assignments n k .. n k + k - 1.  weight NULL: 1; else of weight_type (32 bits or the rows' type).  A token without active assignments
  * gets zeros.  dst [n_tokens, width] contiguous. */
@@ -59,8 +63,8 @@ int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t
                           int32_t weight_type, const void* src, int64_t src_stride, void* dst, void* stream);
 /* Gradient of rows_combine: d_src[p] = weight[a] * dy[token], zeros behind the last active row; d_weight[a] = <dy[token], src[p]>, 0 for
  * dropped assignments.  Either of d_src / d_weight may be NULL. */
-int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_t* assign, const int32_t* row_token, const void* weight, int32_t weight_type, const void* dy,
-                       int64_t dy_stride, const void* src, int64_t src_stride, void* d_src, void* d_weight, void* stream);
+int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_t* row_token, const int32_t* assign, const int32_t* place, const int32_t* token_assign,
+                       const void* weight, int32_t weight_type, const void* dy, int64_t dy_stride, const void* src, int64_t src_stride, void* d_src, void* d_weight, void* stream);
 
 /* The experts' products.  Rows offsets[e] .. offsets[e + 1] - 1 belong to expert e; weight [n_experts, out, inp] and bias [n_experts, out] (NULL: none) are
  * contiguous.  y = act(x weight[e]^T + bias[e]) [n_rows, out] contiguous, zeros in the rows behind offsets[n_experts].  z, where not NULL, receives the

@@ -31,7 +31,7 @@ def tiny(dt):
 
 
 def close(got, want, bound, what):
-    got = got.detach().cpu().double()
+    got = got.detach().to(want.device).double()
     assert got.shape == want.shape, what
     bad = ~((got - want).abs() <= bound)
     assert not bad.any(), '%s: %d of %d beyond the bound, worst %g over %g' % (
@@ -79,19 +79,19 @@ def test_c_entries_refuse_before_any_launch():
 
     def refused(rc, word):
         assert rc != 0 and word in L.ccsp_ops_last_error().decode(), L.ccsp_ops_last_error()
-    refused(L.ccsp_ops_route(ok, None, 16, 4, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), '32 or 64')
-    refused(L.ccsp_ops_route(ok, None, 32, 5, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'tokens of 2 each')
-    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 0, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'experts')
-    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 1025, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'experts')
-    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 3, None), 'workspace')
-    refused(L.ccsp_ops_route(ok, ok, 32, 4, 0, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'token_ptr')
-    refused(L.ccsp_ops_route(None, None, 32, 4, 2, 8, 2, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'null')
+    refused(L.ccsp_ops_route(ok, None, 16, 4, 2, 8, 2, ok, ok, ok, ok, ok, None, None, ok, 1 << 20, None), '32 or 64')
+    refused(L.ccsp_ops_route(ok, None, 32, 5, 2, 8, 2, ok, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'tokens of 2 each')
+    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 0, 2, ok, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'experts')
+    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 1025, 2, ok, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'experts')
+    refused(L.ccsp_ops_route(ok, None, 32, 4, 2, 8, 2, ok, ok, ok, ok, ok, None, None, ok, 3, None), 'workspace')
+    refused(L.ccsp_ops_route(ok, ok, 32, 4, 0, 8, 2, ok, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'token_ptr')
+    refused(L.ccsp_ops_route(None, None, 32, 4, 2, 8, 2, ok, ok, ok, ok, ok, None, None, ok, 1 << 20, None), 'null')
     assert L.ccsp_ops_route_workspace(-1, 4, 4, 0) == -1 and L.ccsp_ops_route_workspace((1 << 30) + 1, 4, 4, 0) == -1
-    refused(L.ccsp_ops_rows_gather(7, 4, 4, ok, 4, ok, ok, None), 'type')
-    refused(L.ccsp_ops_rows_gather(0, 4, 4, ok, 4, None, ok, None), 'null')
-    refused(L.ccsp_ops_rows_gather(0, -1, 4, ok, 4, ok, ok, None), 'range')
+    refused(L.ccsp_ops_rows_gather(7, 4, 4, ok, 4, ok, ok, ok, None, ok, None), 'type')
+    refused(L.ccsp_ops_rows_gather(0, 4, 4, ok, 4, None, ok, ok, None, ok, None), 'null')
+    refused(L.ccsp_ops_rows_gather(0, -1, 4, ok, 4, ok, ok, ok, None, ok, None), 'range')
     refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, ok, 2, ok, 4, ok, None), 'weights')
-    refused(L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, 2, ok, 4, ok, 4, ok, ok, None), 'weights')
+    refused(L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, None, ok, 2, ok, 4, ok, 4, ok, ok, None), 'weights')
     refused(L.ccsp_ops_linear(0, 4, 4, 0, 4, ok, ok, 4, ok, None, 0, ok, None, None, 0, None), 'range')
     refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, ok, None, 5, ok, None, None, 0, None), 'activation')
     refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, None, ok, 4, ok, None, 0, ok, None, None, 0, None), 'null')
@@ -319,6 +319,34 @@ def test_sort_and_combine_with_gradients(device, N, k, E, D, dtype, form, layout
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_rows_larger_than_the_last_level_cache(device, dtype):
+    """200 MB of rows and more, which are written past the cache; dropped rows among them"""
+    dt, N, k, E = DTYPES[dtype], 16384, 8, 20
+    D = 512 if dt == torch.float32 else 1024
+    expert = ids(N * k, E, 1, 0.1).reshape(N, k).to(device)
+    plan = ops.route(expert, E)
+    g = torch.Generator(device=device).manual_seed(0)
+    x, gy = torch.randn(N, D, generator=g, device=device).to(dt), torch.randn(N, D, generator=g, device=device).to(dt)
+    ys, w = torch.randn(N * k, D, generator=g, device=device).to(dt).requires_grad_(), torch.randn(N, k, generator=g, device=device).requires_grad_()
+    n = int(plan.offsets[-1])
+    a = plan.assign[:n].long()
+    xs = ops.sort_rows(x, plan)
+    assert torch.equal(xs[:n], x[a // k]) and float(xs[n:].abs().max()) == 0.0 and 0 < n < N * k
+    y = ops.combine_rows(ys, plan, w)
+    d_ys, d_w = torch.autograd.grad(y, [ys, w], gy)
+    W, G, Y = w.detach().reshape(-1)[a].double()[:, None], gy[a // k].double(), ys.detach()[:n].double()
+    want = torch.zeros(N, D, dtype=torch.float64, device=device).index_add_(0, a // k, Y * W)
+    mag = torch.zeros(N, D, dtype=torch.float64, device=device).index_add_(0, a // k, (Y * W).abs())
+    close(y, want, u(dt) * want.abs() + 2 * (k + 1) * U32 * mag + tiny(dt), 'y')
+    close(d_ys[:n], G * W, (u(dt) + 2 * U32) * (G * W).abs() + tiny(dt), 'd ys')
+    assert float(d_ys[n:].abs().max()) == 0.0
+    want_w, mag_w = torch.zeros(N * k, dtype=torch.float64, device=device), torch.zeros(N * k, dtype=torch.float64, device=device)
+    want_w[a], mag_w[a] = (G * Y).sum(1), (G * Y).abs().sum(1)
+    close(d_w.reshape(-1), want_w, 2 * (D + 1) * U32 * mag_w + tiny(torch.float32), 'd weights')
+
+
+@pytest.mark.gpu
 def test_rows_keep_infinities_and_nan_of_active_rows_only(device):
     expert = torch.tensor([[0, 1], [1, -1], [-1, -1]])
     plan = ops.route(expert.to(device), 2)
@@ -341,7 +369,8 @@ def linear_case(counts, tail, I, O, dt, seed):
     return expert, xs, w, bias, gy
 
 
-def check_linear(device, counts, tail, I, O, dt, act, with_bias, layout='plain', seed=0):
+def check_linear(device, counts, tail, I, O, dt, act, with_bias, layout='plain', seed=0, where='cpu'):
+    """where: the device that works out the 64-bit reference (large cases: the GPU's own 64-bit products)"""
     expert, xs, w, bias, gy = linear_case(counts, tail, I, O, dt, seed)
     R, E = sum(counts), len(counts)
     xs_, gy_ = xs.clone(), gy.clone()
@@ -354,10 +383,10 @@ def check_linear(device, counts, tail, I, O, dt, act, with_bias, layout='plain',
     with torch.no_grad():
         assert torch.equal(ops.expert_linear(xd, wd, plan, bd, act), y)          # (the form that keeps no pre-activation)
     lo = 0
-    want_y, by = torch.zeros(R + tail, O, dtype=torch.float64), torch.zeros(R + tail, O, dtype=torch.float64)
-    want_x, bx = torch.zeros(R + tail, I, dtype=torch.float64), torch.zeros(R + tail, I, dtype=torch.float64)
-    want_w, bw = torch.zeros(E, O, I, dtype=torch.float64), torch.zeros(E, O, I, dtype=torch.float64)
-    want_b, bb = torch.zeros(E, O, dtype=torch.float64), torch.zeros(E, O, dtype=torch.float64)
+    xs, w, bias, gy = (t.to(where) for t in (xs, w, bias, gy))
+    zeros = lambda *s: torch.zeros(s, dtype=torch.float64, device=where)      # noqa: E731
+    want_y, by, want_x, bx = zeros(R + tail, O), zeros(R + tail, O), zeros(R + tail, I), zeros(R + tail, I)
+    want_w, bw, want_b, bb = zeros(E, O, I), zeros(E, O, I), zeros(E, O), zeros(E, O)
     for e, n in enumerate(counts):
         s = slice(lo, lo + n)
         lo += n
@@ -399,6 +428,14 @@ LINEAR = [([1], 0, 1, 1), ([0, 3, 0], 1, 8, 8), ([1, 1, 1, 1], 0, 64, 40), ([5, 
 @pytest.mark.parametrize('act,with_bias', [(None, False), (None, True), ('silu', True), ('silu', False)])
 def test_expert_linear_with_gradients(device, counts, tail, I, O, dtype, act, with_bias):
     check_linear(device, counts, tail, I, O, DTYPES[dtype], act, with_bias, seed=I + O)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('counts,tail,I,O', [([900, 0, 1100, 37], 5, 1032, 776), ([13000, 7001], 9, 2056, 4104), ([9000, 1, 0, 3999], 0, 2050, 4100)])
+def test_expert_linear_in_its_larger_tiles(device, counts, tail, I, O, dtype):
+    """enough rows and columns for the 128 x 128 and 256 x 256 tiles, groups and matrices that end inside one, rows that are not whole 16-byte pieces"""
+    check_linear(device, counts, tail, I, O, DTYPES[dtype], 'silu', True, where=device)
 
 
 @pytest.mark.gpu
