@@ -7,13 +7,14 @@ import ctypes
 import math
 import os
 import re
+import sys
 import threading
 
 import numpy as np
 import pytest
 import torch
 
-from conftest import ROOT
+from conftest import ROOT, worlds
 from diffusion_ccsp_amd import CcspError, _ops
 from diffusion_ccsp_amd import operators as ops
 
@@ -681,7 +682,7 @@ def test_a_routed_layer_trains_like_its_plain_form(device):
         rows.append(acc)
     want = torch.stack(rows)
     want.square().sum().backward()
-    assert float((y.detach().cpu().double() - want).abs().max()) <= 1e-4 * float(want.detach().abs().max())
+    assert float((y.detach().cpu().double() - want.detach()).abs().max()) <= 1e-4 * float(want.detach().abs().max())
     for t, r in zip(leaves, ref):
         assert float((t.grad.cpu().double() - r.grad).abs().max()) <= 1e-4 * float(r.grad.abs().max())
     norm = ops.clip_grad_norm_(leaves, 0.1)
@@ -774,3 +775,41 @@ def test_two_graphs_do_not_share_workspaces(device):
         torch.cuda.synchronize()
         for _, plan, want, _, _ in graphs:
             assert torch.equal(plan.rows, want.rows) and torch.equal(plan.assign, want.assign) and torch.equal(plan.offsets, want.offsets)
+
+
+@pytest.mark.gpu
+def test_the_training_command_on_operators_equals_its_plain_form(device, monkeypatch):
+    """tools/train_gpu.py: loss and gradients of the denoiser on the operators against its loop over the types, both in 32 bits on the GPU.  A gradient entry is a sum
+    of at most some thousand rounded terms down a chain of seven layers: 2e-4 of the largest entry of its tensor is an order above the 32-bit spread"""
+    monkeypatch.setenv('TRAIN_DEVICE', 'cuda:0')
+    monkeypatch.setenv('TRAIN_HIDDEN', '64')
+    monkeypatch.setenv('TRAIN_OPERATORS', '1')
+    monkeypatch.syspath_prepend(os.path.join(ROOT, 'tools'))
+    monkeypatch.delitem(sys.modules, 'train_gpu', raising=False)
+    import train_gpu as tg
+    assert tg.USE_OPERATORS
+    rng = np.random.default_rng(4)
+    worlds_ = [worlds.sample_qualitative_world(rng, int(rng.integers(2, 9))) for _ in range(24)]
+    batch = worlds.collate([worlds.encode_qualitative(w['nodes'], w['constraints']) for w in worlds_])
+    torch.manual_seed(1)
+    net = tg.Denoiser().to(device)
+    sa, sb = tg.schedule_tables()
+    b = tg.to_dev(batch)
+    noise, t = torch.randn(batch.x.shape[0], 4, device=device), torch.tensor([300], device=device)
+    results = []
+    for form in ('operators', 'operators', 'plain'):
+        bb = dict(b, nodes=None) if form == 'plain' else b
+        net.zero_grad(set_to_none=True)
+        loss = tg.loss_on(net, bb, t, noise, sa, sb)
+        loss.backward()
+        results.append((loss.detach(), {n: None if p.grad is None else p.grad.clone() for n, p in net.named_parameters()}))
+    (l0, g0), (l1, g1), (l2, g2) = results
+    assert abs(float(l0) - float(l2)) <= 1e-5 * float(l2)
+    for name in g0:
+        # a type without edges: no gradient from the loop, zeros from its group
+        want = torch.zeros_like(g0[name]) if g2[name] is None else g2[name]
+        assert float((g0[name] - want).abs().max()) <= 2e-4 * max(float(want.abs().max()), 1e-6), name
+    norm = ops.clip_grad_norm_(net.parameters(), 0.01)
+    total = math.sqrt(sum(float((g.double() ** 2).sum()) for g in g2.values() if g is not None))
+    assert abs(float(norm) - total) <= 1e-3 * total
+    monkeypatch.delitem(sys.modules, 'train_gpu', raising=False)

@@ -10,6 +10,10 @@ conditioned rows, l2), Adam lr 5e-4, batch 128 graphs (train_utils.py:217-218) -
 package's RandomSplitQualitativeWorld generator.  Output: reference state_dict key names, type-MLP matrices
 int8 row-quantised like the fixtures (the dequantised values ARE the weights).
 
+On the GPU the denoiser runs on the package's own operators (diffusion_ccsp_amd.operators: the edges sorted by constraint type, one product per type, the results
+combined onto the nodes), which makes a step faster and repeatable; TRAIN_OPERATORS=0 keeps the plain torch form (a loop over the types and an atomic
+index_add).  TRAIN_CLIP=<norm> clips the global gradient norm before every step (the reference recipe does not clip).
+
 usage: python tools/train_gpu.py <minutes> <out.npz> [hidden_dim]
 
 TRAIN_RECIPE=reference: the reference's recipe AS WRITTEN for input_mode 'qualitative' (train_utils.py:87,142-156,217-218;
@@ -28,7 +32,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from diffusion_ccsp_amd import worlds
+from diffusion_ccsp_amd import operators, worlds
 
 # TRAIN_DEVICE=cpu lets the build container import this file (oracle/check_train_gpu.py cross-checks it against the
 # reference's own p_losses there); training runs use the GPU
@@ -38,6 +42,8 @@ minutes = float(sys.argv[1]) if _cli else 0.0
 out_path = sys.argv[2] if _cli else ''
 H = int(sys.argv[3]) if _cli and len(sys.argv) > 3 else int(os.environ.get('TRAIN_HIDDEN', '256'))
 T, C, P, BATCH = 1000, 13, 4, 128
+USE_OPERATORS = dev.type == 'cuda' and os.environ.get('TRAIN_OPERATORS', '1') not in ('', '0')
+CLIP = float(os.environ.get('TRAIN_CLIP', '0') or 0)
 dims = worlds.MODE_DIMS['qualitative']
 
 
@@ -61,6 +67,9 @@ class Denoiser(nn.Module):
         g = self.geom_encoder(b['x'][:, :dims[0][2]])
         p = self.pose_encoder(poses)
         te = self.temb(t)                                  # [1, H]
+        if b['nodes'] is not None:
+            out = self.typed_edges(g, p, te, b) / torch.sqrt(b['cnt'])[:, None]
+            return torch.where(b['mask'][:, None], b['x'][:, -P:], out)
         out = torch.zeros_like(poses)
         for i in range(C):
             a0, a1 = b['ea'][i], b['eb'][i]
@@ -73,6 +82,16 @@ class Denoiser(nn.Module):
         out = out / torch.sqrt(b['cnt'])[:, None]
         m = b['mask']
         return torch.where(m[:, None], b['x'][:, -P:], out)
+
+
+    def typed_edges(self, g, p, te, b):
+        """the loop over the constraint types as operators: both nodes' embeddings of every edge in the order of the types (an edge's two rows follow each
+        other), one product per type -- the time embedding is one row, so its columns go into the bias --, the decoder, the sum over a node's edges"""
+        pair = lambda e: operators.sort_rows(e, b['nodes']).reshape(-1, 2 * H)      # noqa: E731
+        w = torch.stack([m[0].weight for m in self.mlps])
+        bias = torch.stack([m[0].bias for m in self.mlps]) + (w[:, :, 4 * H:] @ te[0])
+        h = operators.expert_linear(torch.cat([pair(g), pair(p)], dim=1), w[:, :, :4 * H], b['edges'], bias, 'silu')
+        return operators.combine_rows(self.pose_decoder(h.reshape(-1, H)), b['nodes'])
 
 
 def to_dev(batch):
@@ -89,6 +108,12 @@ def to_dev(batch):
         d['eb'].append(e1[bounds[i]:bounds[i + 1]])
     cnt = np.bincount(ei.reshape(-1), minlength=batch.x.shape[0]).astype(np.float32)
     d['cnt'] = torch.from_numpy(cnt).to(dev, non_blocking=True)
+    d['nodes'] = d['edges'] = None
+    if USE_OPERATORS:
+        kind = torch.from_numpy(np.ascontiguousarray(ea)).to(dev)
+        ends = torch.from_numpy(np.ascontiguousarray(ei.T.astype(np.int64))).to(dev)
+        d['edges'] = operators.route(kind, C)
+        d['nodes'] = operators.route(kind[:, None].expand(-1, 2), C, tokens=ends, n_tokens=batch.x.shape[0])
     return d
 
 
@@ -152,6 +177,8 @@ def main():
         loss = loss_on(net, b, t, torch.randn_like(b['x'][:, dims[-1][1]:dims[-1][2]]), sa, sb)
         opt.zero_grad(set_to_none=True)
         loss.backward()
+        if CLIP > 0:
+            operators.clip_grad_norm_(net.parameters(), CLIP) if USE_OPERATORS else torch.nn.utils.clip_grad_norm_(net.parameters(), CLIP)
         opt.step()
         run = 0.99 * run + 0.01 * loss.item() if step % 50 == 0 and step else run
         if step in ckpts:
