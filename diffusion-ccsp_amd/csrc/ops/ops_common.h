@@ -16,7 +16,7 @@ int fail(const char* fmt, ...) {
         if (_e != hipSuccess) return fail("%s failed: %s (%s:%d)", #expr, hipGetErrorString(_e), __FILE__, __LINE__); \
     } while (0)
 #define CCSP_OPS_CHECK(cond, ...) do { if (!(cond)) return fail(__VA_ARGS__); } while (0)
-// a launch reports through hipGetLastError; an error another call of the host left behind is not this entry's to report
+// an error that is pending when a call comes in is reported by it, as by any HIP call
 #define LAUNCHED() HIP_TRY(hipGetLastError())
 
 typedef __bf16 bf16;

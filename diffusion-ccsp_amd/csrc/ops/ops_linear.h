@@ -516,18 +516,23 @@ __global__ __launch_bounds__(256) void k_join_parts(ProdArgs p) {
     }
 }
 
-// rows of any width, stride and address as rows of whole 16-byte pieces, zeros behind the width
+// rows of any width, stride and address as rows of whole 16-byte pieces, zeros behind the width; y: operand (both in one launch)
+struct PadJob { const void* src; long rows; int width; long stride; void* dst; int pieces; };
 template <typename T>
-__global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ src, long rows, int width, long stride, T* __restrict__ dst, int pieces) {
+__global__ __launch_bounds__(256) void k_pad_rows(PadJob j0, PadJob j1) {
+    const PadJob p = blockIdx.y ? j1 : j0;
     constexpr int V = 16 / sizeof(T);
-    const long n = rows * pieces;
-    for (long i = block_id() * 256 + threadIdx.x; i < n; i += (long)gridDim.x * gridDim.y * 256) {
-        const long r = i / pieces;
-        const int c = (int)(i - r * pieces) * V;
+    const long n = p.rows * p.pieces;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+        const long r = i / p.pieces;
+        const int c = (int)(i - r * p.pieces) * V;
+        const T* const src = static_cast<const T*>(p.src) + r * p.stride;
         union { T e[V]; u32x4 v; } x;
 #pragma unroll
-        for (int j = 0; j < V; ++j) x.e[j] = c + j < width ? src[r * stride + c + j] : (T)0.0f;
-        *reinterpret_cast<u32x4*>(dst + i * V) = x.v;
+        for (int j = 0; j < V; ++j) { const int k = c + j < p.width ? c + j : p.width - 1; x.e[j] = src[k]; }      // (loads without conditions: all in flight)
+#pragma unroll
+        for (int j = 0; j < V; ++j) if (c + j >= p.width) x.e[j] = (T)0.0f;
+        *reinterpret_cast<u32x4*>(static_cast<T*>(p.dst) + i * V) = x.v;
     }
 }
 
@@ -554,7 +559,7 @@ int launch_tiles(const ProdArgs& p, hipStream_t s) {
     const long tn = cdiv(p.N, TN), tm = PROD == PROD_WEIGHT ? cdiv(p.M, TM) : most_tiles(p.R, p.E, Log2<TM>::v);
     const bool cut = PROD == PROD_WEIGHT && p.seg_log2 != 31;
     const long blocks = (PROD == PROD_WEIGHT ? (cut ? most_tiles(p.R, p.E, p.seg_log2) : p.E) : 1) * tm * tn;
-    if (blocks > 0x003fffffL) return fail("expert_linear: %ld tiles are more than a launch holds", blocks);
+    if (blocks * 64 * WM * WN > 0xffffffffL) return fail("expert_linear: %ld tiles are more than a launch holds", blocks);
     if (blocks) hipLaunchKernelGGL((k_product<T, PROD, TM, TN, WM, WN, NST>), dim3((unsigned)blocks), dim3(64 * WM * WN), NST * (TM + TN) * 128, s, p, (int)tm, (int)tn);
     if (cut) {
         const bool four = p.pieces >= 4 && p.M % 4 == 0;
@@ -585,13 +590,15 @@ int prod_tile(bool weight, long R, long E, long M, long N) {
 
 // Rows of a segment of the weight gradient (log2; 31: uncut).  An expert's tile is one block's chain over all of its rows, so a few long experts would
 // leave most CUs idle: rows are cut until there are about four blocks a CU.  A segment's partial sums cost 8 bytes a value to write and add, which
-// its products have to be worth.
+// its products have to be worth: in 32 bits (20264 rows, 13 experts, 512 x 1024, some experts thrice as long as others) 352 -> 200 us; in 16 bits not where one expert alone
+// has a tile for every other CU (8192 rows, 32 experts, 1408 x 2048: 113 us cut, 94 uncut).
 template <typename T>
 int seg_log2_for(long R, long E, long M, long N) {
     const int tile = prod_tile<T>(true, R, E, M, N);
     if (tile == TILE_256) return 31;
     const int least = sizeof(T) == 4 ? 9 : 10;
-    const long want = R * cdiv(M, 1l << tile) * cdiv(N, 1l << tile) / 1024;
+    const long tiles = cdiv(M, 1l << tile) * cdiv(N, 1l << tile), want = R * tiles / 1024;
+    if (sizeof(T) == 2 && tiles >= 128) return 31;
     int l = least;
     while (l < 30 && (2l << l) <= want) ++l;
     return (1l << l) >= R ? 31 : l;
@@ -620,17 +627,22 @@ struct Operand {
     }
     long padded() const { constexpr long V = 16 / sizeof(T); return (width + V - 1) / V * V; }
     int64_t bytes() const { return fits() ? 0 : (rows * padded() * (long)sizeof(T) + 255) & ~255l; }
-    // in place of the operand: where it is and its stride; advances the workspace
-    void place(const void** at, long* ld, char** ws, hipStream_t s) const {
+    // where the product reads it and its stride; the copy that makes it so, if one is needed; advances the workspace
+    PadJob place(const void** at, long* ld, char** ws) const {
         *at = p; *ld = stride;
-        if (fits()) return;
-        const int pieces = (int)(padded() * (long)sizeof(T) / 16);
-        const long blocks = cdiv(rows * pieces, 256);
-        if (blocks) hipLaunchKernelGGL(k_pad_rows<T>, grid_of(blocks < 16384 ? blocks : 16384), dim3(256), 0, s, (const T*)p, rows, (int)width, stride, (T*)*ws, pieces);
+        if (fits()) return {};
+        const PadJob j = {p, rows, (int)width, stride, *ws, (int)(padded() * (long)sizeof(T) / 16)};
         *at = *ws; *ld = padded();
         *ws += bytes();
+        return j;
     }
 };
+template <typename T>
+void pad_rows(PadJob a, PadJob b, hipStream_t s) {
+    if (a.rows == 0) { a = b; b = {}; }
+    const long blocks = cdiv((a.rows * a.pieces > b.rows * b.pieces ? a.rows * a.pieces : b.rows * b.pieces), 256);
+    if (blocks) hipLaunchKernelGGL(k_pad_rows<T>, dim3((unsigned)(blocks < 16384 ? blocks : 16384), b.rows ? 2 : 1), dim3(256), 0, s, a, b);
+}
 template <typename T>
 int result_pieces(long N, long ldc, const void* c, const void* z, const void* bias) {
     const int b = common_align({(uint64_t)N * sizeof(T), (uint64_t)ldc * sizeof(T), (uint64_t)(uintptr_t)c, (uint64_t)(uintptr_t)z, (uint64_t)(uintptr_t)bias}) / (int)sizeof(T);
@@ -668,8 +680,8 @@ int run_product(ProdArgs p, int64_t inp, int64_t out, const void* a, int64_t a_s
     char* ws = static_cast<char*>(workspace);
     Operand<T> oa, ob;
     linear_operands<T>(product, p.E, p.R, inp, out, a, a_stride, b, b_stride, &oa, &ob);
-    oa.place(&p.a, &p.lda, &ws, s);
-    ob.place(&p.b, &p.ldb, &ws, s);
+    const PadJob ja = oa.place(&p.a, &p.lda, &ws), jb = ob.place(&p.b, &p.ldb, &ws);
+    pad_rows<T>(ja, jb, s);
     p.b_expert = (PROD == PROD_WEIGHT ? 0 : out) * p.ldb;
     p.parts = reinterpret_cast<float*>(ws);
     p.pieces = result_pieces<T>(p.N, p.ldc, p.c, p.z, p.bias);

@@ -332,7 +332,8 @@ __global__ __launch_bounds__(512) void k_route_small(RouteIds r, RouteOut o, int
         for (int t = threadIdx.x; t <= r.N; t += 512) o.token_ptr[t] = route_bound(r, o.token_assign, t);
 }
 
-inline int bits_for(long keys) { int b = 0; while ((1l << b) < keys) ++b; return b; }        // digits that hold `keys` values
+// bits that hold `keys` values; one at least, so that every sort has a pass (no tokens: one key, and everything is dropped)
+inline int bits_for(long keys) { int b = 1; while ((1l << b) < keys) ++b; return b; }
 
 // ints of workspace: histograms of one pass of each sort, two orders between passes of the token sort
 inline size_t route_workspace_ints(long A, int E, long N, bool list) {

@@ -339,11 +339,24 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
         if (!out) to[i] = const_cast<void*>(from[i]);
     }
     if (max_norm) {
-        std::vector<void*> used;
-        used.reserve(n);
-        for (size_t i = 0; i < n; ++i) if (sizes[i]) used.push_back(out ? to[i] : src[i].data_ptr());
-        std::sort(used.begin(), used.end());
-        VALUE(std::adjacent_find(used.begin(), used.end()) == used.end(), who, ": a tensor to write appears twice");
+        // what is written may lie on nothing else, except that an output may be its own gradient
+        struct Run { const char *lo, *hi; size_t i; bool in; };
+        std::vector<Run> runs;
+        runs.reserve(2 * n);
+        for (size_t i = 0; i < n; ++i) {
+            if (!sizes[i]) continue;
+            const int64_t bytes = sizes[i] * (types[i] == CCSP_OPS_F32 ? 4 : 2);
+            const char* const w = (const char*)(out ? to[i] : src[i].data_ptr());
+            runs.push_back({w, w + bytes, i, false});
+            if (out && from[i] != to[i]) runs.push_back({(const char*)from[i], (const char*)from[i] + bytes, i, true});
+        }
+        std::sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) { return a.lo < b.lo; });
+        const char *end = nullptr, *end_written = nullptr;       // of everything, of what is written, up to here
+        for (const Run& r : runs) {
+            VALUE(r.lo >= (r.in ? end_written : end), who, ": a tensor to write appears twice or lies on another tensor");
+            end = std::max(end, r.hi);
+            if (!r.in) end_written = std::max(end_written, r.hi);
+        }
     }
     const int64_t need = ccsp_ops_norm_workspace((int32_t)n, sizes.data());
     const Tensor res = at::empty({2}, src[0].options().dtype(at::kFloat)), ws = at::empty({need}, src[0].options().dtype(at::kByte));

@@ -202,6 +202,55 @@ def test_route_of_nothing(device):
 
 
 @pytest.mark.gpu
+def test_assignments_of_no_tokens(device):
+    """listed tokens of an empty layer: everything is dropped, every result is there and zero"""
+    expert, tokens = torch.zeros((6, 2), dtype=torch.int64, device=device), torch.zeros((6, 2), dtype=torch.int64, device=device)
+    plan = ops.route(expert, 3, tokens=tokens, n_tokens=0)
+    check_plan(plan, expert.cpu(), 3, tokens.cpu(), 0, True)
+    for D in (0, 5, 256):
+        x = torch.zeros((0, D), device=device, requires_grad=True)
+        ys = torch.full((12, D), float('nan'), device=device, requires_grad=True)
+        w = torch.ones((6, 2), device=device, requires_grad=True)
+        xs, y = ops.sort_rows(x, plan), ops.combine_rows(ys, plan, w)
+        assert tuple(y.shape) == (0, D) and float(xs.detach().abs().sum()) == 0.0
+        for g in torch.autograd.grad([xs, y], [x, ys, w], [torch.ones_like(xs), torch.ones_like(y)]):
+            assert float(g.abs().sum()) == 0.0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(device):
+    """more than 2^31 elements (and more than 2^32 bytes) before the rows that are looked at: the last ones"""
+    R, D, I = 1100000, 2048, 64
+    g = torch.Generator(device=device).manual_seed(0)
+    expert = (torch.arange(R, device=device) % 3)[:, None]
+    plan = ops.route(expert, 3)
+    x = torch.randn(R, D, generator=g, device=device, dtype=torch.float16)
+    xs = ops.sort_rows(x, plan)
+    p = torch.arange(R - 5000, R, device=device)
+    tok = plan.row_token[p].long()
+    assert torch.equal(xs[p], x[tok])
+    y = ops.combine_rows(xs, plan)
+    assert torch.equal(y[-5000:], x[-5000:])
+    del xs, y
+    small = torch.randn(R, I, generator=g, device=device, dtype=torch.float16).requires_grad_()
+    w = (torch.randn(3, D, I, generator=g, device=device) / 8).half().requires_grad_()
+    z = ops.expert_linear(small, w, plan)
+    d_small, d_w = torch.autograd.grad(z, [small, w], x)
+    s64, w64, x64 = small.detach()[p].double(), w.detach()[2].double(), x[p].double()        # (the last rows are expert 2's)
+    want = s64 @ w64.t()
+    close(z[p], want, u(torch.float16) * want.abs() + 2 * (I + 1) * U32 * (s64.abs() @ w64.abs().t()) + tiny(torch.float16), 'y')
+    want = x64 @ w64
+    close(d_small[p], want, u(torch.float16) * want.abs() + 2 * (D + 1) * U32 * (x64.abs() @ w64.abs()) + tiny(torch.float16), 'd xs')
+    r = slice(int(plan.offsets[2]), R)
+    want, mag = torch.zeros(D, I, dtype=torch.float64, device=device), torch.zeros(D, I, dtype=torch.float64, device=device)
+    for lo in range(r.start, R, 50000):
+        a, b = x[lo:min(lo + 50000, R)].double(), small.detach()[lo:min(lo + 50000, R)].double()
+        want += a.t() @ b
+        mag += a.abs().t() @ b.abs()
+    close(d_w[2], want, u(torch.float16) * want.abs() + 2 * (R - r.start + 1) * U32 * mag + tiny(torch.float16), 'd weight')
+
+
+@pytest.mark.gpu
 def test_route_refusals(device):
     e = torch.zeros((4, 2), dtype=torch.int64, device=device)
     with pytest.raises(TypeError, match='int32 or int64'):
@@ -633,6 +682,13 @@ def test_clip_grad_norm_of_parameters(device):
     assert ps[0].grad._version > v and ps[3].grad is None
     with pytest.raises(ValueError, match='twice'):
         ops.clip_global_norm([ps[0].grad, ps[0].grad], 1.0)
+    a, b = torch.ones(8, device=device), torch.ones(8, device=device)
+    for grads, out in (([a[:5], a[4:]], None), ([a, b], [b, a]), ([a], [a.clone()[1:].new_zeros(8)]), ([a[:4], b[:4]], [a[2:6], b[:4]]), ([a[:4], a[4:]], [b[4:], b[:4]])):
+        if out is None or out[0].data_ptr() in (b.data_ptr(), a[2:].data_ptr()):
+            with pytest.raises(ValueError, match='lies on another'):
+                ops.clip_global_norm(grads, 1.0, out=out)
+        else:
+            ops.clip_global_norm(grads, 1.0, out=out)
     with pytest.raises(ValueError, match='negative'):
         ops.clip_global_norm([ps[0].grad], -1.0)
     with pytest.raises(ValueError, match='negative'):
@@ -733,7 +789,7 @@ def test_captured_and_replayed(device):
         grads = torch.autograd.grad(y, static, torch.ones_like(y))
         out = [torch.empty_like(t) for t in grads]
         norm = ops.clip_global_norm(grads, 0.25, out=out)
-        return [plan.offsets, y, norm] + out
+        return [plan.offsets, y.detach(), norm] + out
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
