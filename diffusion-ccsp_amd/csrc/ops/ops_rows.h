@@ -15,7 +15,8 @@
 constexpr int ROWS_BY_TOKEN = 512;
 // Results that the last-level cache (256 MB) cannot hold anyway are written past it, which leaves it to the rows that are read again: 32768 tokens x 8, 2048 in
 // bf16 (1 GB): gather 317 -> 194 us, 6.2 TB/s; 65536 x 2, 1024 (268 MB): 79 -> 60; but 4096 x 4, 4096 (134 MB): 27.5 -> 28.8.
-// (back: 449 -> 430 and 129 -> 124 us)
+// (back: 449 -> 430 and 129 -> 124 us.)  The rows that combine reads are read once: past the cache at every size (1 GB: 225 -> 203 us; 83 MB, 20264 typed edges of 512 in
+// 32 bits: 26 -> 21), but only in whole 16-byte accesses -- smaller ones come back for the rest of a line (4099 x 3, 1001 in fp16: 15 -> 20).
 constexpr long ROWS_PAST_CACHE = 192l << 20;
 
 struct RowOrder {
@@ -32,6 +33,8 @@ __device__ __forceinline__ void row_at(const RowOrder& o, long i, int* p, int* t
     *tok = o.row_token[*p];
     *a = pl < 0 ? ~as : as;
 }
+
+template <bool ONCE, typename V> __device__ __forceinline__ V load_once(const V* p) { if constexpr (ONCE) return __builtin_nontemporal_load(p); else return *p; }
 
 template <int VB> struct Chunk;
 template <> struct Chunk<16> { typedef u32x4 t; };
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(256) void k_rows_combine(long n_tokens, int chunks,
 #pragma unroll
             for (int u = 0; u < U; ++u) { row[u] = rows[as[u]]; wt[u] = weight_at<T>(w, wf32, as[u]); }
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const VT*>(src + (row[u] < 0 ? 0 : row[u]) * src_stride + (long)c * V);
+            for (int u = 0; u < U; ++u) v[u] = load_once<V * sizeof(T) == 16>(reinterpret_cast<const VT*>(src + (row[u] < 0 ? 0 : row[u]) * src_stride + (long)c * V));
 #pragma unroll
             for (int u = 0; u < U; ++u) if (j + u >= j1) row[u] = -1;
 #pragma unroll
@@ -128,7 +131,7 @@ __global__ __launch_bounds__(256) void k_rows_back(RowOrder o, long n_rows, int 
         VT g, s, d;
         if (tok >= 0) {
             g = *reinterpret_cast<const VT*>(dy + tok * dy_stride + (long)c * V);
-            if (d_w) s = *reinterpret_cast<const VT*>(src + p * src_stride + (long)c * V);
+            if (d_w) s = load_once<NT>(reinterpret_cast<const VT*>(src + p * src_stride + (long)c * V));
         }
         const T *ge = reinterpret_cast<const T*>(&g), *se = reinterpret_cast<const T*>(&s);
         T* de = reinterpret_cast<T*>(&d);
