@@ -46,7 +46,7 @@ int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t
                           int32_t weight_type, const void* src, int64_t src_stride, void* dst, void* stream) {
     if (check_rows("rows_combine", type, n_tokens, width)) return 1;
     if (n_tokens == 0 || width == 0) return 0;
-    CCSP_OPS_CHECK(dst && (token_ptr || k >= 0), "rows_combine: null argument");
+    CCSP_OPS_CHECK(dst && (token_ptr || (k >= 0 && (k == 0 || (rows && src)))), "rows_combine: null argument");      // (a list may be empty: then nothing is read)
     CCSP_OPS_CHECK(!weight || weight_type == CCSP_OPS_F32 || weight_type == type, "rows_combine: weights are 32 bits or of the rows' type");
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;

@@ -605,9 +605,7 @@ int seg_log2_for(long R, long E, long M, long N) {
 }
 
 template <typename T, int PROD>
-int launch_prod(const ProdArgs& p, hipStream_t s) {
-    constexpr bool W = PROD == PROD_WEIGHT;
-    const int tile = prod_tile<T>(W, p.R, p.E, p.M, p.N);
+int launch_prod(const ProdArgs& p, int tile, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
         if (tile == TILE_256) return launch_tiles<T, PROD, 256, 256, 2, 4, 2>(p, s);
         if (tile == TILE_128) return launch_tiles<T, PROD, 128, 128, 2, 2, 2>(p, s);
@@ -685,5 +683,6 @@ int run_product(ProdArgs p, int64_t inp, int64_t out, const void* a, int64_t a_s
     p.b_expert = (PROD == PROD_WEIGHT ? 0 : out) * p.ldb;
     p.parts = reinterpret_cast<float*>(ws);
     p.pieces = result_pieces<T>(p.N, p.ldc, p.c, p.z, p.bias);
-    return launch_prod<T, PROD>(p, s);
+    // (by the operands, not by p.N: the bias gradient alone is added up in the same order as beside the product)
+    return launch_prod<T, PROD>(p, prod_tile<T>(PROD == PROD_WEIGHT, p.R, p.E, out, PROD == PROD_FORWARD ? out : inp), s);
 }

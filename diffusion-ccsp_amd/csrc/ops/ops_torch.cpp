@@ -345,7 +345,8 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
         runs.reserve(2 * n);
         for (size_t i = 0; i < n; ++i) {
             if (!sizes[i]) continue;
-            const int64_t bytes = sizes[i] * (types[i] == CCSP_OPS_F32 ? 4 : 2);
+            // (a gradient with holes in it is read before anything is written, and may lie between another's elements: only its first one counts)
+            const int64_t bytes = (out || src[i].is_non_overlapping_and_dense() ? sizes[i] : 1) * (types[i] == CCSP_OPS_F32 ? 4 : 2);
             const char* const w = (const char*)(out ? to[i] : src[i].data_ptr());
             runs.push_back({w, w + bytes, i, false});
             if (out && from[i] != to[i]) runs.push_back({(const char*)from[i], (const char*)from[i] + bytes, i, true});

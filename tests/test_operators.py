@@ -92,6 +92,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(L.ccsp_ops_rows_gather(0, 4, 4, ok, 4, None, ok, ok, None, ok, None), 'null')
     refused(L.ccsp_ops_rows_gather(0, -1, 4, ok, 4, ok, ok, ok, None, ok, None), 'range')
     refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, ok, 2, ok, 4, ok, None), 'weights')
+    refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, None, None, 1, ok, 4, ok, None), 'null')
+    refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, None, 1, None, 4, ok, None), 'null')
     refused(L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, None, ok, 2, ok, 4, ok, 4, ok, ok, None), 'weights')
     refused(L.ccsp_ops_linear(0, 4, 4, 0, 4, ok, ok, 4, ok, None, 0, ok, None, None, 0, None), 'range')
     refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, ok, None, 5, ok, None, None, 0, None), 'activation')
@@ -585,6 +587,22 @@ def test_a_frozen_weight_or_input_gets_no_gradient(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('counts,I,O', [([40, 0, 90], 200, 136), ([900, 0, 1100, 37], 1032, 776), ([13000, 7001], 2056, 4104), ([3000, 5000], 300, 200)])
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_the_bias_gradient_alone_has_the_bits_it_has_beside_the_weights(device, counts, I, O, dtype):
+    """over every size of tile, cut into segments and not"""
+    expert = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts)).to(device)
+    plan = ops.route(expert, len(counts))
+    g = torch.Generator(device=device).manual_seed(8)
+    xs, w, bias, gy = [torch.randn(*s, generator=g, device=device).to(DTYPES[dtype]) for s in ((sum(counts), I), (len(counts), O, I), (len(counts), O), (sum(counts), O))]
+    bias.requires_grad_()
+    alone, = torch.autograd.grad(ops.expert_linear(xs, w, plan, bias), bias, gy)
+    w.requires_grad_()
+    beside = torch.autograd.grad(ops.expert_linear(xs, w, plan, bias), (w, bias), gy)[1]
+    assert torch.equal(alone, beside)
+
+
+@pytest.mark.gpu
 def test_a_gradient_of_a_gradient_is_refused(device):
     expert, leaves, E = layer_inputs(device, torch.float32)
     plan = ops.route(expert, E)
@@ -702,6 +720,18 @@ def test_clip_grad_norm_of_parameters(device):
 
 
 # ---- together, as they are used ------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_clip_of_gradients_between_each_others_elements(device):
+    """strided views without a common element are clipped in place, whatever lies between their elements"""
+    x = torch.randn(40, 6, generator=torch.Generator().manual_seed(3))
+    y = x.to(device)
+    host = [x[:, ::2].clone(), x[:, 1].clone(), x[:, 3::2].clone()]
+    got = [y[:, ::2], y[:, 1], y[:, 3::2]]
+    check_clip(ops.clip_global_norm(got, 0.5), got, host, 0.5)
+    with pytest.raises(ValueError, match='twice'):
+        ops.clip_global_norm([got[0], y[:, ::2]], 0.5)
+
 
 def layer(x, plan, w1, b1, w2, weights):
     h = ops.expert_linear(ops.sort_rows(x, plan), w1, plan, b1, 'silu')
