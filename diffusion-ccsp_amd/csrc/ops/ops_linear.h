@@ -21,6 +21,7 @@ struct ProdArgs {
     int E, R, M, N, K;                                           // M, N, K of one expert's product; the one that is a row count is -1
     int silu;
     int pieces;                                                  // elements of a result's row that one access may take: 8, 4 or 1
+    int past;                                                    // the results pass the last-level cache by (in whole pieces)
     float* parts;                                                // weight gradient of experts with more than 2^seg_log2 rows: [slot][M N + M] partial sums
     int seg_log2;                                                // 31: no expert's rows are cut
 };
@@ -400,7 +401,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     if (PROD == PROD_WEIGHT && !p.c) return;                     // (the sums alone)
     if constexpr (!F32) {
         // Whole 16-byte pieces: the wave's part goes through its share of LDS (free since the last barrier), so that a store writes eight rows' runs of
-        // 16 (TN / WN) / 8 bytes instead of sixteen rows' 32: 65536 rows, 16 experts 2048 -> 4096: 1220 -> 1080 us
+        // 16 (TN / WN) / 8 bytes instead of sixteen rows' 32: 65536 rows, 16 experts 2048 -> 4096: 1220 -> 1080 us.  Results that the last-level cache cannot
+        // hold are written past it, as rows are: the same product with its rows evenly spread 1198 -> 1173 us, the weight gradient of 64 experts 2048 -> 1408 (369 MB)
+        // of 2048 rows 117 -> 98; smaller ones gain 2 % at most and are read from the cache next
         if (p.pieces == 8 && !part) {
             constexpr int PM = TM / WM, PN = TN / WN, CH = PN / 8;         // the wave's part, 16-byte pieces of its row
             T* const own = reinterpret_cast<T*>(lds) + wave * PM * PN;
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                     for (int r = 0; r < 4; ++r) bv[j][r] = (float)b[r];
                 }
             }
-            auto out = [&](T* to, bool act) {
+            auto out = [&](T* to, bool act, auto past) {
 #pragma unroll
                 for (int i = 0; i < FA; ++i)
 #pragma unroll
@@ -432,12 +435,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                 for (int it = 0; it < PM * CH / 64; ++it) {
                     const int m = it * (64 / CH) + lane / CH, c = lane % CH, n = n0 + wn + 8 * c;
                     const u32x4 v = *reinterpret_cast<const u32x4*>(own + m * PN + ((c ^ (m & (CH - 1))) << 3));
-                    if (wm + m < left_m && n < N) *reinterpret_cast<u32x4*>(to + (long)(wm + m) * p.ldc + n) = v;
+                    if (wm + m >= left_m || n >= N) continue;
+                    u32x4* const at = reinterpret_cast<u32x4*>(to + (long)(wm + m) * p.ldc + n);
+                    if constexpr (decltype(past)::value) __builtin_nontemporal_store(v, at); else *at = v;
                 }
                 asm volatile("" ::: "memory");
             };
-            out(C, silu);
-            if (Z) out(Z, false);
+            if (p.past) {
+                out(C, silu, std::true_type{});
+                if (Z) out(Z, false, std::true_type{});
+            } else {
+                out(C, silu, std::false_type{});
+                if (Z) out(Z, false, std::false_type{});
+            }
             return;
         }
     }
@@ -683,6 +693,7 @@ int run_product(ProdArgs p, int64_t inp, int64_t out, const void* a, int64_t a_s
     p.b_expert = (PROD == PROD_WEIGHT ? 0 : out) * p.ldb;
     p.parts = reinterpret_cast<float*>(ws);
     p.pieces = result_pieces<T>(p.N, p.ldc, p.c, p.z, p.bias);
+    p.past = (PROD == PROD_WEIGHT ? (long)p.E * p.M : (long)p.R) * p.N * (long)sizeof(T) >= ROWS_PAST_CACHE;
     // (by the operands, not by p.N: the bias gradient alone is added up in the same order as beside the product)
     return launch_prod<T, PROD>(p, prod_tile<T>(PROD == PROD_WEIGHT, p.R, p.E, out, PROD == PROD_FORWARD ? out : inp), s);
 }
