@@ -491,6 +491,14 @@ def test_expert_linear_in_its_larger_tiles(device, counts, tail, I, O, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('counts,tail,I,O', [([15000, 10001], 5, 72, 4104), ([30, 0, 1, 128] * 7, 0, 2056, 2048)])
+def test_expert_linear_with_results_larger_than_the_last_level_cache(device, counts, tail, I, O, dtype):
+    """205 MB of rows, 236 MB of weight gradients: they are written past the cache"""
+    check_linear(device, counts, tail, I, O, DTYPES[dtype], 'silu', False, where=device)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('layout', ['offset', 'columns'])
 @pytest.mark.parametrize('dtype', list(DTYPES))
 def test_expert_linear_on_strided_rows(device, layout, dtype):
