@@ -86,7 +86,7 @@ def lib():
     L.ccsp_ops_route_workspace.restype = i64
     L.ccsp_ops_route.argtypes = [vp, vp, i32, i64, i32, i32, i64] + [vp] * 8 + [i64, vp]
     L.ccsp_ops_rows_gather.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6
-    L.ccsp_ops_rows_combine.argtypes = [i32, i64, i64, i32, vp, vp, vp, vp, i32, vp, i64, vp, vp]
+    L.ccsp_ops_rows_combine.argtypes = [i32, i64, i64, i64, i32, vp, vp, vp, vp, i32, vp, i64, vp, vp]
     L.ccsp_ops_rows_back.argtypes = [i32, i64, i64] + [vp] * 5 + [i32, vp, i64, vp, i64, vp, vp, vp]
     L.ccsp_ops_linear_workspace.argtypes = [i32, i32, i32, i64, i64, i64, vp, i64, vp, i64]
     L.ccsp_ops_linear_workspace.restype = i64

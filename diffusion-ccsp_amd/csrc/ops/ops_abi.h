@@ -38,19 +38,21 @@ int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void
     if (check_rows("rows_gather", type, n_rows, width)) return 1;
     if (n_rows == 0 || width == 0) return 0;
     CCSP_OPS_CHECK(row_token && assign && place && dst, "rows_gather: null argument");
-    const long b = type_bytes(type);
-    return rows_gather({row_token, assign, place, token_assign}, n_rows, width * b, src, src_stride * b, dst, width * b, (hipStream_t)stream);
+    const long b = type_bytes(type) / 2;
+    return rows_gather({row_token, assign, place, token_assign}, n_rows, (int)(width * b), src, src_stride * b, dst, width * b, (hipStream_t)stream);
 }
 
-int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
+int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t n_rows, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
                           int32_t weight_type, const void* src, int64_t src_stride, void* dst, void* stream) {
-    if (check_rows("rows_combine", type, n_tokens, width)) return 1;
+    if (check_rows("rows_combine", type, n_tokens, width) || check_rows("rows_combine", type, n_rows, width)) return 1;
+    CCSP_OPS_CHECK(token_ptr || n_rows == n_tokens * k, "rows_combine: %lld rows are not %lld tokens of %d each (list tokens need token_ptr)", (long long)n_rows, (long long)n_tokens, k);
     if (n_tokens == 0 || width == 0) return 0;
-    CCSP_OPS_CHECK(dst && (token_ptr || (k >= 0 && (k == 0 || (rows && src)))), "rows_combine: null argument");      // (a list may be empty: then nothing is read)
+    CCSP_OPS_CHECK(dst && (n_rows == 0 || (rows && src)), "rows_combine: null argument");
+    CCSP_OPS_CHECK(!token_ptr || n_rows == 0 || token_assign, "rows_combine: list tokens need token_assign");
     CCSP_OPS_CHECK(!weight || weight_type == CCSP_OPS_F32 || weight_type == type, "rows_combine: weights are 32 bits or of the rows' type");
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;
-        return rows_combine<T>(n_tokens, (int)width, k, token_ptr, token_assign, rows, weight, weight_type == CCSP_OPS_F32, (const T*)src, src_stride, (T*)dst, width, (hipStream_t)stream);
+        return rows_combine<T>(n_tokens, n_rows, (int)width, k, token_ptr, token_assign, rows, weight, weight_type == CCSP_OPS_F32, (const T*)src, src_stride, (T*)dst, width, (hipStream_t)stream);
     });
 }
 
@@ -102,10 +104,10 @@ int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, i
     CCSP_OPS_CHECK(dy && z && dz, "linear_silu_back: null argument");
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;
-        dispatch_vec<T>(rows_vec<T>(out, {dy, z, dz}, {dy_stride}), [&](auto vc) {
+        dispatch_vec<sizeof(T)>(out, [&](auto vc) {
             constexpr int V = decltype(vc)::value;
-            const long n = cdiv(n_rows * (out / V), 256);
-            hipLaunchKernelGGL((k_silu_back<T, V>), dim3((unsigned)(n < 8192 ? n : 8192)), dim3(256), 0, (hipStream_t)stream, offsets + n_experts, (int)(out / V), (const T*)dy, (long)dy_stride, (const T*)z,
+            const long n = cdiv(n_rows * cdiv(out, V), 256);
+            hipLaunchKernelGGL((k_silu_back<T, V>), dim3((unsigned)(n < 8192 ? n : 8192)), dim3(256), 0, (hipStream_t)stream, offsets + n_experts, (int)out, (const T*)dy, (long)dy_stride, (const T*)z,
                                (T*)dz);
         });
         LAUNCHED();

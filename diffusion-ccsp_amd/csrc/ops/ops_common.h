@@ -28,6 +28,9 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, int N> struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
 template <typename T> struct VecOf<T, 1> { typedef T type; };
+// N elements at any element's address: one access of 16 bytes needs no alignment (the target's unaligned access mode, which the compiler counts on for such a type)
+template <typename T, int N> struct LooseOf { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+template <typename T> struct LooseOf<T, 1> { typedef T type; };
 
 // one block per item: a grid's x holds 2^32 threads, so large counts spread over y (the last row of blocks may run past the count)
 inline dim3 grid_of(long blocks) { return blocks <= (1l << 22) ? dim3((unsigned)blocks) : dim3(1u << 22, (unsigned)((blocks + (1l << 22) - 1) >> 22)); }

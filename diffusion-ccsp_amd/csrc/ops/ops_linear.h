@@ -537,11 +537,17 @@ __global__ __launch_bounds__(256) void k_pad_rows(PadJob j0, PadJob j1) {
         const long r = i / p.pieces;
         const int c = (int)(i - r * p.pieces) * V;
         const T* const src = static_cast<const T*>(p.src) + r * p.stride;
-        union { T e[V]; u32x4 v; } x;
+        union { T e[V]; unsigned long h[2]; u32x4 v; } x;
+        if (p.width >= V) {                                      // the last piece ends with the row and is moved down
+            const int at = c + V <= p.width ? c : p.width - V, by = (c - at) * 8 * (int)sizeof(T);
+            const typename LooseOf<T, V>::type v = *reinterpret_cast<const typename LooseOf<T, V>::type*>(src + at);
+            __builtin_memcpy(&x, &v, 16);
+            if (by >= 64) { x.h[0] = x.h[1] >> (by - 64); x.h[1] = 0; }
+            else if (by > 0) { x.h[0] = x.h[0] >> by | x.h[1] << (64 - by); x.h[1] >>= by; }
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) { const int k = c + j < p.width ? c + j : p.width - 1; x.e[j] = src[k]; }      // (loads without conditions: all in flight)
-#pragma unroll
-        for (int j = 0; j < V; ++j) if (c + j >= p.width) x.e[j] = (T)0.0f;
+            for (int j = 0; j < V; ++j) x.e[j] = j < p.width ? src[j] : (T)0.0f;
+        }
         *reinterpret_cast<u32x4*>(static_cast<T*>(p.dst) + i * V) = x.v;
     }
 }
@@ -549,18 +555,19 @@ __global__ __launch_bounds__(256) void k_pad_rows(PadJob j0, PadJob j1) {
 // ---- around the products -------------------------------------------------------------------------------------------------
 // dz = dy silu'(z) over the active rows (z as it was stored: its rounding moves the slope by less than dz's own rounding does)
 template <typename T, int V>
-__global__ __launch_bounds__(256) void k_silu_back(const int* __restrict__ active, int chunks, const T* __restrict__ dy, long dy_stride, const T* __restrict__ z, T* __restrict__ dz) {
-    typedef typename VecOf<T, V>::type VT;
+__global__ __launch_bounds__(256) void k_silu_back(const int* __restrict__ active, int width, const T* __restrict__ dy, long dy_stride, const T* __restrict__ z, T* __restrict__ dz) {
+    typedef typename LooseOf<T, V>::type VT;
+    const int chunks = (width + V - 1) / V;
     const long n = (long)active[0] * chunks;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-        const long r = i / chunks, c = i - r * chunks;
-        const VT g = *reinterpret_cast<const VT*>(dy + r * dy_stride + c * V), zz = *reinterpret_cast<const VT*>(z + i * V);
+        const long r = i / chunks, c = access_at<V>((int)(i - r * chunks), width);
+        const VT g = *reinterpret_cast<const VT*>(dy + r * dy_stride + c), zz = *reinterpret_cast<const VT*>(z + r * width + c);
         const T *ge = reinterpret_cast<const T*>(&g), *ze = reinterpret_cast<const T*>(&zz);
         VT o;
         T* oe = reinterpret_cast<T*>(&o);
 #pragma unroll
         for (int j = 0; j < V; ++j) oe[j] = (T)((float)ge[j] * silu_slope<T>((float)ze[j]));
-        *reinterpret_cast<VT*>(dz + i * V) = o;
+        *reinterpret_cast<VT*>(dz + r * width + c) = o;
     }
 }
 

@@ -104,44 +104,36 @@ __global__ __launch_bounds__(1024) void k_norm_finish(const double* part, long n
     }
 }
 
+// (accesses start where p is a multiple of 16; o may lie otherwise)
 template <typename T>
 __device__ __forceinline__ void clip_chunk(const T* p, T* o, long n, float c) {
     constexpr int V = 16 / sizeof(T);
     typedef typename VecOf<T, V>::type VT;
-    long done = 0;
-    if ((((uintptr_t)p ^ (uintptr_t)o) & 15) == 0) {             // both reach 16 bytes together
-        const long head_all = (16 - ((uintptr_t)p & 15) & 15) / sizeof(T), head = head_all < n ? head_all : n;
-        if ((long)threadIdx.x < head) o[threadIdx.x] = (T)((float)p[threadIdx.x] * c);
-        const VT* q = reinterpret_cast<const VT*>(p + head);
-        VT* r = reinterpret_cast<VT*>(o + head);
-        const long nv = (n - head) / V;
-        long i = threadIdx.x;
-        for (; i + 768 < nv; i += 1024) {
-            VT x[4];
+    typedef typename LooseOf<T, V>::type OT;
+    const long head_all = (16 - ((uintptr_t)p & 15) & 15) / sizeof(T), head = head_all < n ? head_all : n;
+    if ((long)threadIdx.x < head) o[threadIdx.x] = (T)((float)p[threadIdx.x] * c);
+    const VT* q = reinterpret_cast<const VT*>(p + head);
+    OT* r = reinterpret_cast<OT*>(o + head);
+    const long nv = (n - head) / V;
+    long i = threadIdx.x;
+    for (; i + 768 < nv; i += 1024) {                            // four accesses in flight
+        VT x[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = q[i + 256 * u];
+        for (int u = 0; u < 4; ++u) x[u] = q[i + 256 * u];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 4; ++u) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[u][j] = (T)((float)x[u][j] * c);
-                r[i + 256 * u] = x[u];
-            }
+            for (int j = 0; j < V; ++j) x[u][j] = (T)((float)x[u][j] * c);
+            r[i + 256 * u] = x[u];
         }
-        for (; i < nv; i += 256) {
-            VT x = q[i];
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * c);
-            r[i] = x;
-        }
-        done = head + nv * V;
     }
-    for (long t = done + threadIdx.x; t < n; t += 2048) {        // (all of the chunk where the two are aligned differently)
-        float x[8];
+    for (; i < nv; i += 256) {
+        VT x = q[i];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = t + 256 * u < n ? (float)p[t + 256 * u] : 0.0f;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) if (t + 256 * u < n) o[t + 256 * u] = (T)(x[u] * c);
+        for (int j = 0; j < V; ++j) x[j] = (T)((float)x[j] * c);
+        r[i] = x;
     }
+    for (long t = head + nv * V + threadIdx.x; t < n; t += 256) o[t] = (T)((float)p[t] * c);
 }
 
 __global__ __launch_bounds__(256) void k_norm_clip(NormTable t, int blocks, const float* scale) {

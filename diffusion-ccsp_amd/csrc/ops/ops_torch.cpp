@@ -122,7 +122,7 @@ Tensor gather(const Tensor& src_in, const Plan& q) {
 Tensor combine(const Tensor& src_in, const Plan& q, const Tensor& weights) {
     On on(src_in);
     const Tensor src = rows_of(src_in), out = at::empty({q.n_tokens, src.size(1)}, src.options());
-    run(ccsp_ops_rows_combine(code(src), q.n_tokens, src.size(1), (int32_t)q.k, q.listed ? q.p(Plan::TOKEN_PTR) : nullptr, q.token_order(), q.p(Plan::ROWS), ptr(weights),
+    run(ccsp_ops_rows_combine(code(src), q.n_tokens, q.n_rows, src.size(1), (int32_t)q.k, q.listed ? q.p(Plan::TOKEN_PTR) : nullptr, q.token_order(), q.p(Plan::ROWS), ptr(weights),
                               weights.defined() ? code(weights) : CCSP_OPS_F32, ptr(src), src.stride(0), ptr(out), on.stream));
     return out;
 }

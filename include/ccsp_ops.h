@@ -58,8 +58,8 @@ int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void
                          const int32_t* token_assign, void* dst, void* stream);
 /* dst[n] = sum over the token's active assignments a, ascending, of weight[a] * src[rows[a]]; sums in 32 bits, rounded once.  token_ptr /
  * token_assign NULL: assignments n k .. n k + k - 1.  weight NULL: 1; else of weight_type (32 bits or the rows' type).  A token without active assignments
- * gets zeros.  dst [n_tokens, width] contiguous. */
-int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
+ * gets zeros.  src: n_rows rows.  dst [n_tokens, width] contiguous. */
+int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t n_rows, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
                           int32_t weight_type, const void* src, int64_t src_stride, void* dst, void* stream);
 /* Gradient of rows_combine: d_src[p] = weight[a] * dy[token], zeros behind the last active row; d_weight[a] = <dy[token], src[p]>, 0 for
  * dropped assignments.  Either of d_src / d_weight may be NULL. */

@@ -91,9 +91,11 @@ def test_c_entries_refuse_before_any_launch():
     refused(L.ccsp_ops_rows_gather(7, 4, 4, ok, 4, ok, ok, ok, None, ok, None), 'type')
     refused(L.ccsp_ops_rows_gather(0, 4, 4, ok, 4, None, ok, ok, None, ok, None), 'null')
     refused(L.ccsp_ops_rows_gather(0, -1, 4, ok, 4, ok, ok, ok, None, ok, None), 'range')
-    refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, ok, 2, ok, 4, ok, None), 'weights')
-    refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, None, None, 1, ok, 4, ok, None), 'null')
-    refused(L.ccsp_ops_rows_combine(1, 4, 4, 2, None, None, ok, None, 1, None, 4, ok, None), 'null')
+    refused(L.ccsp_ops_rows_combine(1, 4, 8, 4, 2, None, None, ok, ok, 2, ok, 4, ok, None), 'weights')
+    refused(L.ccsp_ops_rows_combine(1, 4, 8, 4, 2, None, None, None, None, 1, ok, 4, ok, None), 'null')
+    refused(L.ccsp_ops_rows_combine(1, 4, 8, 4, 2, None, None, ok, None, 1, None, 4, ok, None), 'null')
+    refused(L.ccsp_ops_rows_combine(1, 4, 7, 4, 2, None, None, ok, None, 1, ok, 4, ok, None), 'tokens of 2 each')
+    refused(L.ccsp_ops_rows_combine(1, 4, 7, 4, 0, ok, None, ok, None, 1, ok, 4, ok, None), 'token_assign')
     refused(L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, None, ok, 2, ok, 4, ok, 4, ok, ok, None), 'weights')
     refused(L.ccsp_ops_linear(0, 4, 4, 0, 4, ok, ok, 4, ok, None, 0, ok, None, None, 0, None), 'range')
     refused(L.ccsp_ops_linear(0, 4, 4, 4, 4, ok, ok, 4, ok, None, 5, ok, None, None, 0, None), 'activation')
