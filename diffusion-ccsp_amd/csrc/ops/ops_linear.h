@@ -132,14 +132,19 @@ struct Stager {
             }
         }
     }
-    // `left` > 0 of k from here on
-    __device__ __forceinline__ void load(unsigned int lds, int left) {
+    __device__ __forceinline__ u32x4 rsrc(int k) const {         // k of the stage are there
         u32x4 r;
         r[0] = __builtin_amdgcn_readfirstlane((unsigned int)base);
         r[1] = __builtin_amdgcn_readfirstlane((unsigned int)(base >> 32) & 0xffffu);
-        r[2] = KC ? 0x7fffffffu : (unsigned int)__builtin_amdgcn_readfirstlane((left < SK ? left : SK) * row_bytes);
+        r[2] = KC ? 0x7fffffffu : (unsigned int)__builtin_amdgcn_readfirstlane(k * row_bytes);
         r[3] = 0x00020000u;
-        const unsigned int to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * N * 1024);
+        return r;
+    }
+    __device__ __forceinline__ unsigned int place(unsigned int lds) const { return __builtin_amdgcn_readfirstlane(lds + (threadIdx.x >> 6) * N * 1024); }
+    // the next stage to LDS address `lds`: `left` > 0 of k from here on
+    __device__ __forceinline__ void load(unsigned int lds, int left) {
+        const u32x4 r = rsrc(left < SK ? left : SK);
+        const unsigned int to = place(lds);
         if (KC && left < SK) {
 #pragma unroll
             for (int i = 0; i < N; ++i) lds_dma16(r, kk < left ? off[i] : DMA_OUT, to + i * 1024);
@@ -148,6 +153,12 @@ struct Stager {
             for (int i = 0; i < N; ++i) lds_dma16(r, off[i], to + i * 1024);
         }
         base += step;
+    }
+    // the same piece by piece without a branch, i = 0 .. N - 1 in turn; left may be <= 0
+    __device__ __forceinline__ void load_piece(unsigned int lds, int left, int i) {
+        const int k = left < SK ? left : SK;
+        lds_dma16(rsrc(left > 0 ? k : 0), !KC || kk < left ? off[i] : DMA_OUT, place(lds) + i * 1024);
+        if (i == N - 1) base += step;
     }
 };
 
@@ -221,6 +232,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     constexpr int G = F32 ? 32 : 16, FA = TM / WM / G, FB = TN / WN / G, RG = F32 ? 16 : 4;      // fragment side, fragments, result registers
     constexpr int SK = 128 / sizeof(T), STAGE = (TM + TN) * SK;
     constexpr int KS = F32 ? 4 : 2;                              // k steps of a stage
+    constexpr bool SPREAD = TM * TN == 65536 && PROD != PROD_WEIGHT;
     typedef typename VecOf<float, RG>::type Acc;
     typedef typename std::conditional<F32, f32x4, typename Vec8<T>::t>::type Frag;
     extern __shared__ __attribute__((aligned(16))) unsigned short lds[];
@@ -275,42 +287,58 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
             ga.load(l0 + buf * BYTES, K - st * SK);
             gb.load(l0 + buf * BYTES + TM * 128, K - st * SK);
         };
+        auto piece = [&](int st, int buf, int i) {               // 0 .. L - 1 in turn
+            if (i < ga.N) ga.load_piece(l0 + buf * BYTES, K - st * SK, i);
+            else gb.load_piece(l0 + buf * BYTES + TM * 128, K - st * SK, i - ga.N);
+        };
 #pragma unroll
-        for (int i = 0; i < NST; ++i) if (i < stages) fetch(i, i);
+        for (int i = 0; i < NST; ++i) {
+            if constexpr (SPREAD) {
+#pragma unroll
+                for (int l = 0; l < L; ++l) piece(i, i, l);
+            } else if (i < stages) fetch(i, i);
+        }
         // A wave multiplies one k step while the next one's fragments come out of LDS; at a stage's last step those are the next stage's, so that is where it
         // has to be there.  Its loads come back in order: NST - 2 later stages may still be on their way.  The barrier makes it everyone's part of
         // the stage, and says that nobody reads this stage any more (its reads have come back): the loads for the stage NST further go into its place.
+        // In one burst these fill the queue that the LDS reads wait in too.  The rows' products in the largest tile have them among their matrix instructions, without a
+        // condition (behind the last stage they ask for nothing and write zeros): 16384 rows, 1 expert 4096 -> 4096: forward 440 -> 390 us, input gradient 420 -> 391.
+        // The weight gradient gains nothing from it (405: its reads are twice as many), and smaller tiles have few stages, of which the empty ones are a part (32 experts of
+        // 256 rows, 2048 x 1408: 88 -> 94).
         Frag fa[2][FA], fb[2][FB];
         constexpr int ACROSS = F32 ? 4 : 2, READS = FA * (AKC ? 1 : ACROSS) + FB * (BKC ? 1 : ACROSS);       // LDS reads of a k step
+        auto read_b = [&](int set, const T* sB, int ks, int j) {
+            if constexpr (F32) fb[set][j] = stage_frag32<BKC, TN>(sB, wn + G * j, ks);
+            else fb[set][j] = stage_frag<T, BKC, TN>(sB, wn + G * j, ks);
+        };
+        auto read_a = [&](int set, const T* sA, int ks, int i) {
+            if constexpr (F32) fa[set][i] = stage_frag32<AKC, TM>(sA, wm + G * i, ks);
+            else fa[set][i] = stage_frag<T, AKC, TM>(sA, wm + G * i, ks);
+        };
         auto read = [&](int set, int buf, int ks) {
             const T *sA = sm + buf * STAGE, *sB = sA + TM * SK;
 #pragma unroll
-            for (int j = 0; j < FB; ++j) {
-                if constexpr (F32) fb[set][j] = stage_frag32<BKC, TN>(sB, wn + G * j, ks);
-                else fb[set][j] = stage_frag<T, BKC, TN>(sB, wn + G * j, ks);
-            }
+            for (int j = 0; j < FB; ++j) read_b(set, sB, ks, j);
 #pragma unroll
-            for (int i = 0; i < FA; ++i) {
-                if constexpr (F32) fa[set][i] = stage_frag32<AKC, TM>(sA, wm + G * i, ks);
-                else fa[set][i] = stage_frag<T, AKC, TM>(sA, wm + G * i, ks);
-            }
+            for (int i = 0; i < FA; ++i) read_a(set, sA, ks, i);
         };
         auto loop = [&](auto with_sums) {
             constexpr bool S = decltype(with_sums)::value;
+            auto multiply_row = [&](int set, int i, int k) {
+#pragma unroll
+                for (int j = 0; j < FB; ++j) {
+                    if constexpr (F32) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[set][j][k], fa[set][i][k], acc[i][j], 0, 0, 0);
+                    else acc[i][j] = mfma16(fb[set][j], fa[set][i], acc[i][j]);
+                }
+                if constexpr (F32) { if (S) sum[i] += fa[set][i][k]; }
+            };
             auto multiply = [&](int set) {
 #pragma unroll
                 for (int k = 0; k < (F32 ? 4 : 1); ++k)
 #pragma unroll
-                    for (int i = 0; i < FA; ++i) {
-#pragma unroll
-                        for (int j = 0; j < FB; ++j) {
-                            if constexpr (F32) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[set][j][k], fa[set][i][k], acc[i][j], 0, 0, 0);
-                            else acc[i][j] = mfma16(fb[set][j], fa[set][i], acc[i][j]);
-                        }
-                        if constexpr (F32) { if (S) sum[i] += fa[set][i][k]; }
-                    }
+                    for (int i = 0; i < FA; ++i) multiply_row(set, i, k);
             };
-            if (NST <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
+            if (SPREAD || NST <= stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * L) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
@@ -332,16 +360,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                     multiply(ks & 1);
                     spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
                 }
-                if (st + NST - 1 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * L) : "memory");
+                if (SPREAD || st + NST - 1 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * L) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                if (st + NST < stages) fetch(st + NST, buf);
-                buf = buf + 1 == NST ? 0 : buf + 1;
-                read(0, buf, 0);                                 // (behind the last stage: whatever lies there, unused)
-                asm volatile("" ::: "memory");                   // (or the compiler reads them in the next round after all)
-                multiply((KS - 1) & 1);
-                spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
+                const int freed = buf;
+                if (!SPREAD && st + NST < stages) fetch(st + NST, freed);
+                buf = buf + 1 == NST ? 0 : buf + 1;              // (behind the last stage: whatever lies there, unused)
+                if constexpr (SPREAD) {
+                    const T *sA = sm + buf * STAGE, *sB = sA + TM * SK;
+#pragma unroll
+                    for (int g = 0; g < FA; ++g) {
+#pragma unroll
+                        for (int f = g * (FA + FB) / FA; f < (g + 1) * (FA + FB) / FA; ++f) if (f < FB) read_b(0, sB, 0, f); else read_a(0, sA, 0, f - FB);
+#pragma unroll
+                        for (int l = g * L / FA; l < (g + 1) * L / FA; ++l) piece(st + NST, freed, l);
+                        __builtin_amdgcn_s_setprio(1);           // (a wave with products before one that asks for data)
+                        multiply_row((KS - 1) & 1, g, 0);
+                        __builtin_amdgcn_s_setprio(0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    asm volatile("" ::: "memory");               // (or the compiler reads them in the next round after all)
+                } else {
+                    read(0, buf, 0);
+                    asm volatile("" ::: "memory");
+                    multiply((KS - 1) & 1);
+                    spread_reads<READS, FA * FB * (F32 ? 4 : 1)>();
+                }
                 if constexpr (F32) {
                     if ((st + 1) % FLUSH == 0) {
                         asm volatile("" ::: "memory");          // (a branch, not 48 selects every stage)
@@ -353,6 +398,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                         }
                     }
                 }
+            }
+            if constexpr (SPREAD) {                              // (the loads for stages that are not there write zeros: the LDS is free behind them)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
             }
         };
         if (F32 && PROD == PROD_WEIGHT && sums) loop(std::true_type{}); else loop(std::false_type{});
@@ -591,17 +641,19 @@ int launch_tiles(const ProdArgs& p, hipStream_t s) {
 
 // Tiles of a product by how many there are: 256 x 256 where they fill the CUs, 128 x 128, and 64 x 64 with four stages where even those are too few to
 // keep enough bytes on their way (one token's experts, short prompts).  Measured in bf16, 128 against 256:
-//   rows x outputs: 8192 rows, 1 expert, 4096 -> 4096 (528 tiles of 256): 282 us against 244; 20264 rows, 13 experts, 2048 -> 2048 (736): 181 against 166;
-//   but 16384 rows, 16 experts, 2048 -> 2048 (640): 150 against 162: at 1024 rows an expert an eighth of the 256-row tiles is empty
-//   weight gradient: 8192 rows, 1 expert, 4096 x 4096 (256 tiles): 260 against 228; 32768 rows, 8 experts, 2048 x 1024 (256): 188 against 128; but 32 experts of
-//   256 rows, 2048 x 1408: 110 against 128: few rows an expert write more than they multiply, and a CU's two small blocks do one while the other does the other
+//   rows x outputs: 8192 rows, 1 expert, 4096 -> 4096 (528 tiles of 256): 279 us against 215; 20264 rows, 13 experts, 2048 -> 2048 (736): 187 against 166; 8192 rows,
+//   8 experts, 4096 -> 4096 (656): 310 against 283; 16384 rows, 16 experts, 2048 -> 2048 (640): 148 both, and below: at 1024 rows an expert an eighth of
+//   the 256-row tiles is empty; 8192 rows, 32 experts, 2048 -> 1408 (390): 64 against 93
+//   weight gradient: 8192 rows, 1 expert, 4096 x 4096 (256 tiles): 281 against 248; 32768 rows, 8 experts, 2048 x 1024 (256): 129 against 110; 16384 rows, 12 experts,
+//   2048 x 2048 (768): 139 against 132; but 20264 rows, 13 experts (832): 174 against 188, three rounds of the CUs and a quarter; 32 experts of 256 rows, 2048 x 1408: 81 against
+//   82, uneven ones 110 against 128: few rows an expert write more than they multiply, and a CU's two small blocks do one while the other does the other
 inline long prod_tiles(bool weight, long R, long E, long M, long N, int l) { return (weight ? E * cdiv(M, 1l << l) : most_tiles(R, E, l)) * cdiv(N, 1l << l); }
 enum { TILE_64 = 6, TILE_128 = 7, TILE_256 = 8 };
 template <typename T>
 int prod_tile(bool weight, long R, long E, long M, long N) {
     if (sizeof(T) == 4) return TILE_64;
     const long big = prod_tiles(weight, R, E, M, N, 8);
-    if (weight ? big >= 256 && R >= 1024 * E : big >= 1024 || (big >= 512 && R >= 1280 * E)) return TILE_256;
+    if (weight ? big >= 256 && R >= 1024 * E : big >= 1024 || (big >= 512 && R >= 1024 * E)) return TILE_256;
     return prod_tiles(weight, R, E, M, N, 7) >= 512 ? TILE_128 : TILE_64;
 }
 
