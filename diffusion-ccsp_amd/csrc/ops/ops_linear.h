@@ -87,8 +87,8 @@ __device__ __forceinline__ f32x4 mfma16(Vec8<fp16>::t a, Vec8<fp16>::t b, f32x4 
 // 32 bits use v_mfma_f32_32x32x2_f32 (products and sums in 32 bits throughout); its two k are taken 4 apart, so that a lane's k of four instructions are
 // one 16-byte read where k is contiguous.
 //
-// TM x TN by WM x WN waves.  A wave's TM / WM x TN / WN part decides how many LDS bytes a product costs: in 16 bits the LDS port is as
-// busy as the matrix pipe at 64 x 64 and three quarters of it at 128 x 64.
+// TM x TN by WM x WN waves.  A wave's TM / WM x TN / WN part decides how many LDS bytes a product costs: at 128 x 64 (256 x 256 by 2 x 4) in 16 bits the
+// LDS is busy 23 % of the time and the matrix pipe 60.
 // ------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void lds_dma16(u32x4 rsrc, unsigned int offset, unsigned int lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
@@ -451,9 +451,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
     if (PROD == PROD_WEIGHT && !p.c) return;                     // (the sums alone)
     if constexpr (!F32) {
         // Whole 16-byte pieces: the wave's part goes through its share of LDS (free since the last barrier), so that a store writes eight rows' runs of
-        // 16 (TN / WN) / 8 bytes instead of sixteen rows' 32: 65536 rows, 16 experts 2048 -> 4096: 1220 -> 1080 us.  Results that the last-level cache cannot
-        // hold are written past it, as rows are: the same product with its rows evenly spread 1198 -> 1173 us, the weight gradient of 64 experts 2048 -> 1408 (369 MB)
-        // of 2048 rows 117 -> 98; smaller ones gain 2 % at most and are read from the cache next
+        // 16 (TN / WN) / 8 bytes instead of sixteen rows' 32: 65536 rows, 16 experts 2048 -> 4096: 1220 -> 1080 us.  Where the last-level cache cannot
+        // hold operands and result together, results are written past it and leave it to the operands, which other tiles and the next products read again: 8192 rows, 32 experts
+        // 2048 -> 1408 with gradients (184 MB of weights) 286 -> 258 us, of which only the weight gradient past it 277; the weight gradient of 64 experts 2048 -> 1408 of
+        // 2048 rows 117 -> 98 us.  Where all fits, a result is read from the cache next.
         if (p.pieces == 8 && !part) {
             constexpr int PM = TM / WM, PN = TN / WN, CH = PN / 8;         // the wave's part, 16-byte pieces of its row
             T* const own = reinterpret_cast<T*>(lds) + wave * PM * PN;
@@ -752,7 +753,9 @@ int run_product(ProdArgs p, int64_t inp, int64_t out, const void* a, int64_t a_s
     p.b_expert = (PROD == PROD_WEIGHT ? 0 : out) * p.ldb;
     p.parts = reinterpret_cast<float*>(ws);
     p.pieces = result_pieces<T>(p.N, p.ldc, p.c, p.z, p.bias);
-    p.past = (PROD == PROD_WEIGHT ? (long)p.E * p.M : (long)p.R) * p.N * (long)sizeof(T) >= ROWS_PAST_CACHE;
+    // elements read and written: rows on both sides, and the weights or their gradient (of a few rows no more experts than rows are read)
+    const long experts = PROD == PROD_WEIGHT || p.E < p.R ? p.E : p.R;
+    p.past = (p.R * (inp + out) + experts * inp * out) * (long)sizeof(T) >= ROWS_PAST_CACHE;
     // (by the operands, not by p.N: the bias gradient alone is added up in the same order as beside the product)
     return launch_prod<T, PROD>(p, prod_tile<T>(PROD == PROD_WEIGHT, p.R, p.E, out, PROD == PROD_FORWARD ? out : inp), s);
 }
