@@ -36,7 +36,7 @@ def _compile(so, sources, cmd, force, verbose):
 
 def build(force=False, verbose=False):
     """compile both libraries in-tree for gfx950 (cross-compiles without a GPU).  -packed-fp32-ops: no packed 32-bit float instructions, some forms of which have
-    given wrong results on these boards (hipcc's host pass warns that it does not know the feature: harmless)."""
+    given wrong results on MI355X (hipcc's host pass warns that it does not know the feature: harmless)."""
     import sysconfig
     from torch.utils import cpp_extension
     header = os.path.join(CSRC, '..', '..', 'include', 'ccsp_ops.h')
