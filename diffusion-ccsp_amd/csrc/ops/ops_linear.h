@@ -69,6 +69,14 @@ template <typename T> __device__ __forceinline__ float sigmoid_of(float z) {
 template <typename T> __device__ __forceinline__ float silu_value(float z) { return sizeof(T) == 4 ? z / (1.0f + expf(-z)) : z * sigmoid_of<T>(z); }
 template <typename T> __device__ __forceinline__ float silu_slope(float z) { const float s = sigmoid_of<T>(z); return s * (1.0f + z * (1.0f - s)); }
 
+// A pre-activation as it is kept for the gradient: one that is finite in 32 bits stays finite in the type, or the slope of silu, 0 or 1 that far out, would be NaN (0 x inf).
+// (An infinite one stays what it is: the formula's NaN.)
+template <typename T> __device__ __forceinline__ T kept_value(float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    constexpr float most = std::is_same<T, fp16>::value ? 65504.0f : 0x1.fep127f;
+    return (T)(v - v == 0.0f ? __builtin_amdgcn_fmed3f(v, -most, most) : v);
+}
+
 template <typename T> struct Vec8 { typedef T t __attribute__((ext_vector_type(8))); };
 __device__ __forceinline__ f32x4 mfma16(Vec8<bf16>::t a, Vec8<bf16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma16(Vec8<fp16>::t a, Vec8<fp16>::t b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -471,7 +479,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                     for (int r = 0; r < 4; ++r) bv[j][r] = (float)b[r];
                 }
             }
-            auto out = [&](T* to, bool act, auto past) {
+            auto out = [&](T* to, bool act, auto keep, auto past) {
 #pragma unroll
                 for (int i = 0; i < FA; ++i)
 #pragma unroll
@@ -479,7 +487,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                         const int m = G * i + (lane & 15), c = 2 * j + (lane >> 5);
                         V4 y;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) { const float v = acc[i][j][r] + bv[j][r]; y[r] = act ? (T)silu_value<T>(v) : (T)v; }
+                        for (int r = 0; r < 4; ++r) {
+                            const float v = acc[i][j][r] + bv[j][r];
+                            if constexpr (decltype(keep)::value) y[r] = kept_value<T>(v); else y[r] = act ? (T)silu_value<T>(v) : (T)v;
+                        }
                         *reinterpret_cast<V4*>(own + m * PN + ((c ^ (m & (CH - 1))) << 3) + 4 * (lane >> 4 & 1)) = y;
                     }
                 asm volatile("" ::: "memory");                   // (a wave's LDS accesses keep their order; other lanes wrote what a lane reads)
@@ -494,11 +505,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
                 asm volatile("" ::: "memory");
             };
             if (p.past) {
-                out(C, silu, std::true_type{});
-                if (Z) out(Z, false, std::true_type{});
+                out(C, silu, std::false_type{}, std::true_type{});
+                if (Z) out(Z, false, std::true_type{}, std::true_type{});
             } else {
-                out(C, silu, std::false_type{});
-                if (Z) out(Z, false, std::false_type{});
+                out(C, silu, std::false_type{}, std::false_type{});
+                if (Z) out(Z, false, std::true_type{}, std::false_type{});
             }
             return;
         }
@@ -532,7 +543,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float v = acc[i][j][4 * g + r] + bv[r];
-                    z[r] = (T)v;
+                    z[r] = kept_value<T>(v);
                     y[r] = silu ? (T)silu_value<T>(v) : (T)v;
                 }
                 const long at = (long)m * p.ldc + n;

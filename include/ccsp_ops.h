@@ -68,7 +68,7 @@ int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_
 
 /* The experts' products.  Rows offsets[e] .. offsets[e + 1] - 1 belong to expert e; weight [n_experts, out, inp] and bias [n_experts, out] (NULL: none) are
  * contiguous.  y = act(x weight[e]^T + bias[e]) [n_rows, out] contiguous, zeros in the rows behind offsets[n_experts].  z, where not NULL, receives the
- * pre-activation of the active rows (what silu_back reads).  Products and sums in 32 bits.
+ * pre-activation of the active rows (what silu_back reads; a finite one beyond the type's range as the type's largest value).  Products and sums in 32 bits.
  * workspace (each of the three products): ccsp_ops_linear_workspace bytes, aligned to 16, for the same operands: copies of operands whose rows are not whole
  * 16-byte pieces at multiples of 16 bytes, and partial sums of the weight gradient.  Often 0; -1: an argument is out of range. */
 enum { CCSP_OPS_FORWARD = 0 /* a = x, b = weight */, CCSP_OPS_BACK_INPUT = 1 /* a = dz, b = weight */, CCSP_OPS_BACK_WEIGHT = 2 /* a = dz, b = x */ };

@@ -909,3 +909,71 @@ def test_the_training_command_on_operators_equals_its_plain_form(device, monkeyp
     total = math.sqrt(sum(float((g.double() ** 2).sum()) for g in g2.values() if g is not None))
     assert abs(float(norm) - total) <= 1e-3 * total
     monkeypatch.delitem(sys.modules, 'train_gpu', raising=False)
+
+
+# ---- values past a 16-bit type's range -----------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('O', [24, 25])
+@pytest.mark.parametrize('counts', [[5, 0, 9], [9000, 1, 0, 3999]])
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_silu_gradient_of_pre_activations_past_the_types_range(device, counts, O, dtype):
+    """Pre-activations that are finite in 32 bits and infinite in the rows' type, of both signs: the slope there is 0 or 1.  All values are powers of two or short sums of
+    them.  Columns 0 and 1 make the large pre-activation, which lies 0.1 % and more past the type's largest value: what the sigmoid leaves of it is 0 on the
+    negative side, 1 on the other, in 32 and 64 bits alike.  The other columns are zero, so every product below is one term and exact up to its own rounding"""
+    dt, I, E = DTYPES[dtype], 16, len(counts)
+    g = torch.Generator().manual_seed(2)
+    R = sum(counts)
+    a, b = (1024.0, 72.0) if dt == torch.float16 else (2.0 ** 64, 2.0 ** 63 * 1.9921875)
+    x = torch.zeros(R, I, dtype=dt)
+    x[:, 0], x[:, 1], x[:, 2] = a, a, torch.randint(1, 4, (R,), generator=g).to(dt)
+    w = torch.zeros(E, O, I, dtype=dt)
+    w[:, 3, 0], w[:, 3, 1] = -b, -b * 2.0 ** -8                   # 2^127 * 1.9999 is past bfloat16, inside float32; -74016 past float16
+    w[:, 5] = -w[:, 3]
+    w[:, 7, 2] = 1.0                                              # an ordinary one beside them
+    gy = (torch.randint(0, 2, (R, O), generator=g) * 2 - 1).to(dt) * 2.0 ** -6
+    expert = torch.repeat_interleave(torch.arange(E), torch.tensor(counts))
+    plan = ops.route(expert.to(device), E)
+    xd, wd, bd = x.to(device).requires_grad_(), w.to(device).requires_grad_(), torch.zeros(E, O, dtype=dt, device=device, requires_grad=True)
+    y = ops.expert_linear(xd, wd, plan, bd, 'silu')
+    d_x, d_w, d_b = torch.autograd.grad(y, (xd, wd, bd), gy.to(device))
+    z = torch.stack([x[p].double() @ w[e].double().t() for p, e in enumerate(expert.tolist()[:4])])
+    assert (dt == torch.float32) == bool(torch.isfinite(z.to(dt)).all()) and bool(torch.isfinite(z.float()).all())
+    Z = torch.zeros(R, O, dtype=torch.float64)
+    Z[:, 3], Z[:, 5], Z[:, 7] = z[0, 3], z[0, 5], x[:, 2].double()
+    s = torch.sigmoid(Z)
+    got = y.detach().cpu()
+    assert float(got[:, 3].abs().max()) == 0.0 and torch.equal(got[:, 5].double(), Z[:, 5].to(dt).double())
+    slope = s * (1 + Z * (1 - s))
+    assert float(slope[:, 3].abs().max()) == 0.0 and float((slope[:, 5] - 1).abs().max()) == 0.0
+    dz = gy.double() * slope
+    edz = (u(dt) + 64 * U32) * dz.abs() + tiny(dt)                # (z of column 7 is a whole number, exact; the sigmoid's few units of 32 bits, times 1 + |z|)
+    bound = lambda want, e: e + (u(dt) + 2 * U32) * want.abs() + tiny(dt)      # noqa: E731
+    We = w.double()[0]                                            # (every expert has the same)
+    want = dz @ We
+    close(d_x, want, bound(want, edz @ We.abs() + 2 * (O + 1) * U32 * (dz.abs() @ We.abs())), 'd xs')
+    lo = 0
+    for e, n in enumerate(counts):
+        D, ED, X = dz[lo:lo + n], edz[lo:lo + n], x[lo:lo + n].double()
+        lo += n
+        want = D.t() @ X
+        close(d_w[e], want, bound(want, ED.t() @ X.abs() + 2 * (n + 1) * U32 * (D.abs().t() @ X.abs())), 'd weight')
+        want = D.sum(0)
+        close(d_b[e], want, bound(want, ED.sum(0) + 2 * (n + 1) * U32 * D.abs().sum(0)), 'd bias')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_silu_of_infinite_pre_activations_is_the_formulas(device, dtype):
+    """inputs that are infinite themselves: z sigmoid(z) and its slope as the formula gives them, inf or NaN, and nothing of it in other rows"""
+    dt = DTYPES[dtype]
+    x = torch.zeros(3, 8, dtype=dt, device=device)
+    x[0, 0], x[1, 0], x[2, 1] = math.inf, -math.inf, 1.0
+    w = torch.zeros(1, 8, 8, dtype=dt, device=device)
+    w[0, :, 0] = 1.0
+    plan = ops.route(torch.zeros(3, dtype=torch.int64, device=device), 1)
+    x.requires_grad_()
+    y = ops.expert_linear(x, w, plan, None, 'silu')
+    d_x, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert bool((y[0] == math.inf).all()) and bool(y[1].isnan().all()) and bool((y[2] == 0).all())
+    assert bool(d_x[:2, 0].isnan().all()) and bool((d_x[2, 0] == 4.0).all())      # eight slopes of a half
