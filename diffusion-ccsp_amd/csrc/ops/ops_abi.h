@@ -61,6 +61,7 @@ int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_
     if (check_rows("rows_back", type, n_rows, width)) return 1;
     if (n_rows == 0) return 0;
     CCSP_OPS_CHECK(assign && row_token && place && (width == 0 || (d_src || d_weight)), "rows_back: null argument");
+    CCSP_OPS_CHECK(src || !d_weight || width == 0, "rows_back: null argument (the weights' gradient reads src)");
     CCSP_OPS_CHECK((!weight && !d_weight) || weight_type == CCSP_OPS_F32 || weight_type == type, "rows_back: weights are 32 bits or of the rows' type");
     return dispatch_type(type, [&](auto t) {
         typedef decltype(t) T;

@@ -52,6 +52,10 @@ __global__ __launch_bounds__(256) void k_rows_gather(RowOrder o, long n_rows, in
     int row[RU], tok[RU], as;
 #pragma unroll
     for (int u = 0; u < RU; ++u) row_at(o, i0 + u < n_rows ? i0 + u : n_rows - 1, &row[u], &tok[u], &as);
+    if (!src) {                                                  // (no tokens: nothing to read, whatever the plan says)
+#pragma unroll
+        for (int u = 0; u < RU; ++u) tok[u] = -1;
+    }
     for (int c = threadIdx.x & (tpr - 1); c * V < width; c += tpr) {
         const long at = access_at<V>(c, width);
         C v[RU];
@@ -125,6 +129,7 @@ __global__ __launch_bounds__(256) void k_rows_back(RowOrder o, long n_rows, int 
     const bool in = i < n_rows;
     int p, a, tok;
     row_at(o, in ? i : n_rows - 1, &p, &tok, &a);
+    if (!dy) tok = -1;                                           // (no tokens)
     const float wt = a >= 0 ? weight_at<T>(w, wf32, a) : 0.0f;
     float dot = 0.0f;
     for (int c = threadIdx.x & (tpr - 1); c * V < width; c += tpr) {

@@ -52,7 +52,7 @@ int ccsp_ops_route(const void* expert, const void* token, int32_t id_bits, int64
                    int32_t* offsets, int32_t* rows, int32_t* assign, int32_t* row_token, int32_t* place, int32_t* token_ptr, int32_t* token_assign,
                    void* workspace, int64_t workspace_bytes, void* stream);
 
-/* dst[p] = src[row_token[p]] for p < n_rows, zeros where row_token[p] < 0.  dst [n_rows, width] contiguous.  row_token, assign, place, token_assign (NULL without
+/* dst[p] = src[row_token[p]] for p < n_rows, zeros where row_token[p] < 0 and everywhere if src is NULL (no tokens).  dst [n_rows, width] contiguous.  row_token, assign, place, token_assign (NULL without
  * listed tokens): the plan's. */
 int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void* src, int64_t src_stride, const int32_t* row_token, const int32_t* assign, const int32_t* place,
                          const int32_t* token_assign, void* dst, void* stream);
@@ -62,7 +62,7 @@ int ccsp_ops_rows_gather(int32_t type, int64_t n_rows, int64_t width, const void
 int ccsp_ops_rows_combine(int32_t type, int64_t n_tokens, int64_t n_rows, int64_t width, int32_t k, const int32_t* token_ptr, const int32_t* token_assign, const int32_t* rows, const void* weight,
                           int32_t weight_type, const void* src, int64_t src_stride, void* dst, void* stream);
 /* Gradient of rows_combine: d_src[p] = weight[a] * dy[token], zeros behind the last active row; d_weight[a] = <dy[token], src[p]>, 0 for
- * dropped assignments.  Either of d_src / d_weight may be NULL. */
+ * dropped assignments.  Either of d_src / d_weight may be NULL.  dy NULL (no tokens): zeros.  src is read for d_weight alone. */
 int ccsp_ops_rows_back(int32_t type, int64_t n_rows, int64_t width, const int32_t* row_token, const int32_t* assign, const int32_t* place, const int32_t* token_assign,
                        const void* weight, int32_t weight_type, const void* dy, int64_t dy_stride, const void* src, int64_t src_stride, void* d_src, void* d_weight, void* stream);
 

@@ -977,3 +977,39 @@ def test_silu_of_infinite_pre_activations_is_the_formulas(device, dtype):
     d_x, = torch.autograd.grad(y, x, torch.ones_like(y))
     assert bool((y[0] == math.inf).all()) and bool(y[1].isnan().all()) and bool((y[2] == 0).all())
     assert bool(d_x[:2, 0].isnan().all()) and bool((d_x[2, 0] == 4.0).all())      # eight slopes of a half
+
+
+# ---- addresses that are not there ----------------------------------------------------------------------------------------
+
+def test_the_weights_gradient_without_rows_to_read_is_refused():
+    L = _ops.lib()
+    ok = 64                                                       # (never read)
+    assert L.ccsp_ops_rows_back(1, 4, 4, ok, ok, ok, None, None, 1, ok, 4, None, 4, ok, ok, None) != 0
+    assert 'null' in L.ccsp_ops_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('width', [5, 400])
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_rows_of_no_tokens_are_zeros(device, dtype, width):
+    """a source without an address has no rows: zeros, and no access, also where a plan says that there are some"""
+    dt, code, L = DTYPES[dtype], _ops.TYPES[str(DTYPES[dtype])[6:]], _ops.lib()
+    expert = torch.tensor([[1, 0], [0, -1], [2, 2]], device=device)
+    plan = ops.route(expert, 3)
+    place = torch.empty(6, dtype=torch.int32, device=device)
+    rows, assign = plan.rows.cpu().tolist(), plan.assign.cpu().tolist()
+    host = [0] * 6
+    for p, a in enumerate(assign):
+        host[a if a >= 0 else ~a] = p if a >= 0 else ~p
+    assert [p if p >= 0 else -1 for p in host] == rows
+    place.copy_(torch.tensor(host))
+    stream = torch.cuda.current_stream().cuda_stream
+    out = torch.full((6, width), 7.0, dtype=dt, device=device)
+    parts = (plan.row_token.data_ptr(), plan.assign.data_ptr(), place.data_ptr(), None)
+    assert L.ccsp_ops_rows_gather(code, 6, width, None, width, *parts, out.data_ptr(), stream) == 0
+    assert float(out.abs().max()) == 0.0
+    ys, w = torch.ones(6, width, dtype=dt, device=device), torch.ones(6, device=device)
+    out.fill_(7.0)
+    d_w = torch.full((6,), 7.0, device=device)
+    assert L.ccsp_ops_rows_back(code, 6, width, *parts, w.data_ptr(), 0, None, width, ys.data_ptr(), width, out.data_ptr(), d_w.data_ptr(), stream) == 0
+    assert float(out.abs().max()) == 0.0 and float(d_w.abs().max()) == 0.0
