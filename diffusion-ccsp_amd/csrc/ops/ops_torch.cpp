@@ -36,7 +36,10 @@ struct On {
     explicit On(const Tensor& t) : guard(t.device()), stream((void*)c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-void on_gpu(const char* who, const Tensor& t) {
+// what every tensor of a call has to be
+void usable(const char* who, const Tensor& t) {
+    // (a tangent would be lost without a word: the kernels read the values alone)
+    if (t._fw_grad(0).defined()) throw OpsError(text(who, ": forward-mode derivatives are not supported; gradients come through torch.autograd in reverse"));
     if (!t.is_cuda()) throw OpsError(text(who, ": tensors must be on a GPU (got ", t.device(), "); there is no CPU fallback"));
 }
 void same_device(const char* who, const Tensor& a, const Tensor& b) { VALUE(a.device() == b.device(), who, ": tensors on ", a.device(), " and ", b.device()); }
@@ -77,7 +80,7 @@ struct Plan {
 };
 
 std::shared_ptr<Plan> route(const Tensor& expert_in, int64_t n_experts, const MaybeTensor& tokens_in, c10::optional<int64_t> n_tokens) {
-    on_gpu("route", expert_in);
+    usable("route", expert_in);
     TYPE(expert_in.scalar_type() == at::kInt || expert_in.scalar_type() == at::kLong, "route: expert ids must be int32 or int64, got ", name_of(expert_in));
     VALUE(n_experts >= 1 && n_experts <= CCSP_OPS_MAX_EXPERTS, "route: ", n_experts, " experts, supported are 1 to ", CCSP_OPS_MAX_EXPERTS);
     auto q = std::make_shared<Plan>();
@@ -89,7 +92,7 @@ std::shared_ptr<Plan> route(const Tensor& expert_in, int64_t n_experts, const Ma
         q->k = expert_in.dim() == 1 ? 1 : expert_in.size(1);
         VALUE(q->k > 0, "route: no expert per token");
     } else {
-        on_gpu("route", *tokens_in);
+        usable("route", *tokens_in);
         same_device("route", expert_in, *tokens_in);
         VALUE(tokens_in->sizes() == expert_in.sizes() && tokens_in->scalar_type() == expert_in.scalar_type(), "route: tokens ", name_of(*tokens_in), " ", tokens_in->sizes(),
               " and expert ids ", name_of(expert_in), " ", expert_in.sizes(), " differ");
@@ -183,7 +186,7 @@ void float_rows(const char* who, const char* name, const Tensor& t, int64_t n, c
 }
 
 Tensor sort_rows(const Tensor& x, const Plan& q) {
-    on_gpu("sort_rows", x);
+    usable("sort_rows", x);
     same_device("sort_rows", x, q.buf);
     float_rows("sort_rows", "x", x, q.n_tokens, "one row per token");
     if (at::GradMode::is_enabled() && x.requires_grad()) return SortRows::apply(x, q.buf, &q);
@@ -191,12 +194,12 @@ Tensor sort_rows(const Tensor& x, const Plan& q) {
 }
 
 Tensor combine_rows(const Tensor& ys, const Plan& q, const MaybeTensor& weights_in) {
-    on_gpu("combine_rows", ys);
+    usable("combine_rows", ys);
     same_device("combine_rows", ys, q.buf);
     float_rows("combine_rows", "ys", ys, q.n_rows, "one row per assignment");
     Tensor weights;
     if (weights_in) {
-        on_gpu("combine_rows", *weights_in);
+        usable("combine_rows", *weights_in);
         same_device("combine_rows", ys, *weights_in);
         VALUE(weights_in->sizes() == at::IntArrayRef(q.shape), "combine_rows: weights ", weights_in->sizes(), " for expert ids ", at::IntArrayRef(q.shape));
         TYPE(weights_in->scalar_type() == at::kFloat || weights_in->scalar_type() == ys.scalar_type(), "combine_rows: weights of type ", name_of(*weights_in), " for rows of type ",
@@ -273,8 +276,8 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
 };
 
 Tensor expert_linear(const Tensor& xs, const Tensor& weight_in, const Plan& q, const MaybeTensor& bias_in, const c10::optional<std::string>& activation) {
-    on_gpu("expert_linear", xs);
-    on_gpu("expert_linear", weight_in);
+    usable("expert_linear", xs);
+    usable("expert_linear", weight_in);
     same_device("expert_linear", xs, q.buf);
     same_device("expert_linear", xs, weight_in);
     float_rows("expert_linear", "xs", xs, q.n_rows, "one row per assignment");
@@ -284,7 +287,7 @@ Tensor expert_linear(const Tensor& xs, const Tensor& weight_in, const Plan& q, c
     VALUE(weight_in.size(1) <= CCSP_OPS_MAX_FEATURES && weight_in.size(2) <= CCSP_OPS_MAX_FEATURES, "expert_linear: weight ", weight_in.sizes(), " is out of range");
     Tensor bias;
     if (bias_in) {
-        on_gpu("expert_linear", *bias_in);
+        usable("expert_linear", *bias_in);
         same_device("expert_linear", xs, *bias_in);
         VALUE(bias_in->dim() == 2 && bias_in->size(0) == weight_in.size(0) && bias_in->size(1) == weight_in.size(1), "expert_linear: bias must be [", weight_in.size(0), ", ", weight_in.size(1),
               "], got ", bias_in->sizes());
@@ -312,19 +315,19 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
     std::vector<void*> to(n);
     std::vector<int64_t> sizes(n);
     std::vector<int32_t> types(n);
-    on_gpu(who, src[0]);
+    usable(who, src[0]);
     On on(src[0]);
     at::NoGradGuard no;
     for (size_t i = 0; i < n; ++i) {
         const Tensor& t = src[i];
-        on_gpu(who, t);
+        usable(who, t);
         VALUE(t.device() == src[0].device(), who, ": tensors on ", src[0].device(), " and ", t.device());
         types[i] = t.layout() == at::kStrided ? code(t) : -1;
         TYPE(types[i] >= 0, who, ": a tensor of type ", name_of(t), t.layout() == at::kStrided ? "" : ", sparse or blocked", "; supported are dense float32, bfloat16 and float16");
         sizes[i] = t.numel();
         if (out) {
             const Tensor& o = (*out)[i];
-            on_gpu(who, o);
+            usable(who, o);
             VALUE(o.device() == t.device(), who, ": tensors on ", t.device(), " and ", o.device());
             VALUE(o.scalar_type() == t.scalar_type() && o.sizes() == t.sizes(), who, ": out must hold one tensor of the same type and shape per gradient");
             VALUE(o.is_contiguous(), who, ": out must be contiguous");

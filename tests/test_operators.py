@@ -1013,3 +1013,31 @@ def test_rows_of_no_tokens_are_zeros(device, dtype, width):
     d_w = torch.full((6,), 7.0, device=device)
     assert L.ccsp_ops_rows_back(code, 6, width, *parts, w.data_ptr(), 0, None, width, ys.data_ptr(), width, out.data_ptr(), d_w.data_ptr(), stream) == 0
     assert float(out.abs().max()) == 0.0 and float(d_w.abs().max()) == 0.0
+
+
+# ---- calls that would lose something without a word ----------------------------------------------------------------------
+
+def test_the_norm_of_dual_numbers_is_refused():
+    import torch.autograd.forward_ad as forward_ad
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(3), torch.ones(3))
+        for call in (lambda: ops.global_norm([dual]), lambda: ops.clip_global_norm([dual], 1.0), lambda: ops.global_norm([dual[:2]])):
+            with pytest.raises(CcspError, match='forward-mode'):
+                call()
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused(device):
+    import torch.autograd.forward_ad as forward_ad
+    expert, (x, w, b, w2, weights), E = layer_inputs(device, torch.float32)
+    plan = ops.route(expert, E)
+    xs = ops.sort_rows(x, plan)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))      # noqa: E731
+        for call in (lambda: ops.sort_rows(dual(x), plan), lambda: ops.combine_rows(dual(xs), plan, weights), lambda: ops.combine_rows(xs, plan, dual(weights)),
+                     lambda: ops.expert_linear(dual(xs), w, plan, b), lambda: ops.expert_linear(xs, dual(w), plan, b), lambda: ops.expert_linear(xs, w, plan, dual(b)),
+                     lambda: ops.sort_rows(dual(x.clone().requires_grad_()), plan), lambda: ops.sort_rows(dual(x)[:, 1:], plan), lambda: ops.clip_global_norm([x, dual(b)], 1.0),
+                     lambda: ops.clip_global_norm([x], 1.0, out=[dual(x)])):
+            with pytest.raises(CcspError, match='forward-mode'):
+                call()
+        assert torch.equal(ops.sort_rows(x, plan), xs)            # (a tensor without a tangent is what it was)
