@@ -2,7 +2,10 @@
 // Host code only; the kernels are libccsp_ops.so's.  It exists because a call is short: the smallest operators run 3 us on the GPU, and what
 // a call costs its host -- checks, allocations, the autograd node -- is what a user waits for (in Python: 14 us a call, 50 us with its gradient).
 #include <c10/hip/HIPStream.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../../include/ccsp_ops.h"
@@ -38,6 +41,9 @@ struct On {
 
 // what every tensor of a call has to be
 void usable(const char* who, const Tensor& t) {
+    // (a trace records torch's own operations: of a kernel, nothing but the memory that its result goes to)
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch))
+        throw OpsError(text(who, ": cannot be recorded by torch.jit.trace or make_fx; it may be captured into a graph of the GPU's"));
     // (a tangent would be lost without a word: the kernels read the values alone)
     if (t._fw_grad(0).defined()) throw OpsError(text(who, ": forward-mode derivatives are not supported; gradients come through torch.autograd in reverse"));
     if (!t.is_cuda()) throw OpsError(text(who, ": tensors must be on a GPU (got ", t.device(), "); there is no CPU fallback"));
@@ -149,6 +155,7 @@ struct SortRows : torch::autograd::Function<SortRows> {
     static variable_list backward(AutogradContext* c, variable_list g) {
         const bool more = at::GradMode::is_enabled();
         at::NoGradGuard no;
+        usable("sort_rows", g[0]);
         const Plan q = Plan::load(c, c->get_saved_variables()[0]);
         return first_order("sort_rows", more, {combine(g[0], q, Tensor()), Tensor(), Tensor()});
     }
@@ -165,6 +172,7 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
     static variable_list backward(AutogradContext* c, variable_list grads) {
         const bool more = at::GradMode::is_enabled();
         at::NoGradGuard no;
+        usable("combine_rows", grads[0]);
         const auto saved = c->get_saved_variables();
         const Plan q = Plan::load(c, saved[0]);
         const Tensor& weights = saved[2];
@@ -246,6 +254,7 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
     static variable_list backward(AutogradContext* c, variable_list grads) {
         const bool more = at::GradMode::is_enabled();
         at::NoGradGuard no;
+        usable("expert_linear", grads[0]);
         const auto saved = c->get_saved_variables();
         const Plan q = Plan::load(c, saved[0]);
         const Tensor &x = saved[1], &weight = saved[2], &z = saved[3];

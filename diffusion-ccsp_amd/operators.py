@@ -12,7 +12,8 @@ The denoiser is such a layer: an edge of type e sends its two nodes through the 
 
 Tensors live on one GPU, rows in float32, bfloat16 or float16; sums are held in 32 bits and rounded once.  Work goes to the current stream of the tensors'
 device, nothing waits for it, and a call may be captured into a graph (a backward pass through torch.autograd.grad, as nothing may be left to do on the
-leaves' own stream).  The gradients of sort_rows, combine_rows and expert_linear come through torch.autograd (first order, in reverse: forward-mode derivatives raise).  Every operator gives the same bits for the same inputs.
+leaves' own stream).  The gradients of sort_rows, combine_rows and expert_linear come through torch.autograd (first order, in reverse: forward-mode derivatives raise).  torch.jit.trace and make_fx record torch's own
+operations only: an operator raises under them.  Every operator gives the same bits for the same inputs.
 """
 import torch
 

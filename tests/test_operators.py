@@ -1041,3 +1041,48 @@ def test_forward_mode_derivatives_are_refused(device):
             with pytest.raises(CcspError, match='forward-mode'):
                 call()
         assert torch.equal(ops.sort_rows(x, plan), xs)            # (a tensor without a tangent is what it was)
+
+
+def tracers():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    return [lambda f, t: torch.jit.trace(f, t, check_trace=False), lambda f, t: make_fx(f)(t), lambda f, t: make_fx(f, tracing_mode='real', pre_dispatch=True)(t)]
+
+
+@pytest.mark.parametrize('which', range(3))
+def test_a_trace_of_an_operator_is_refused(which):
+    with pytest.raises(CcspError, match='recorded'):
+        tracers()[which](lambda t: ops.global_norm([t]), torch.ones(3))
+    with pytest.raises(CcspError, match='no CPU fallback'):      # (and it is over with the trace)
+        ops.global_norm([torch.ones(3)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('which', range(3))
+def test_traces_of_all_operators_are_refused(device, which):
+    expert, (x, w, b, w2, weights), E = layer_inputs(device, torch.float32)
+    plan = ops.route(expert, E)
+    xs = ops.sort_rows(x, plan)
+    for f, t in ((lambda t: ops.route(t, E).offsets, expert), (lambda t: ops.sort_rows(t, plan), x), (lambda t: ops.combine_rows(xs, plan, t), weights), (lambda t: ops.expert_linear(xs, t, plan), w),
+                 (lambda t: ops.clip_global_norm([t], 1.0), x.clone())):
+        with pytest.raises(CcspError, match='recorded'):
+            tracers()[which](f, t)
+    assert torch.equal(ops.sort_rows(x, plan), xs)
+
+
+@pytest.mark.gpu
+def test_gradients_of_a_trace_or_with_a_tangent_are_refused(device):
+    """the forward before, the backward pass inside"""
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    expert, leaves, E = layer_inputs(device, torch.float32)
+    x, w, b, w2, weights = [t.requires_grad_() for t in leaves]
+    plan = ops.route(expert, E)
+    xs = ops.sort_rows(x, plan)
+    for y, leaf in ((xs, x), (ops.expert_linear(xs.detach(), w, plan, b), w), (ops.combine_rows(xs.detach(), plan, weights), weights)):
+        g = torch.ones_like(y)
+        want, = torch.autograd.grad(y, leaf, g, retain_graph=True)
+        with pytest.raises(RuntimeError, match='recorded'):
+            make_fx(lambda t: torch.autograd.grad(y, leaf, t, retain_graph=True)[0])(g)      # noqa: B023
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match='forward-mode'):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(g, torch.ones_like(g)), retain_graph=True)
+        assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
