@@ -46,6 +46,9 @@ void usable(const char* who, const Tensor& t) {
         throw OpsError(text(who, ": cannot be recorded by torch.jit.trace or make_fx; it may be captured into a graph of the GPU's"));
     // (a tangent would be lost without a word: the kernels read the values alone)
     if (t._fw_grad(0).defined()) throw OpsError(text(who, ": forward-mode derivatives are not supported; gradients come through torch.autograd in reverse"));
+    // (a wrapper -- a distributed or quantised tensor, one inside torch.func's transforms -- has no memory of its own, or memory that means something else)
+    TYPE(t.layout() == at::kStrided, who, ": a tensor that is sparse or blocked; supported are dense ones");
+    TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch() && t.has_storage(), who, ": a tensor that wraps others (a subclass with its own dispatch, a transform's); supported are plain ones");
     if (!t.is_cuda()) throw OpsError(text(who, ": tensors must be on a GPU (got ", t.device(), "); there is no CPU fallback"));
 }
 void same_device(const char* who, const Tensor& a, const Tensor& b) { VALUE(a.device() == b.device(), who, ": tensors on ", a.device(), " and ", b.device()); }
@@ -331,8 +334,8 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
         const Tensor& t = src[i];
         usable(who, t);
         VALUE(t.device() == src[0].device(), who, ": tensors on ", src[0].device(), " and ", t.device());
-        types[i] = t.layout() == at::kStrided ? code(t) : -1;
-        TYPE(types[i] >= 0, who, ": a tensor of type ", name_of(t), t.layout() == at::kStrided ? "" : ", sparse or blocked", "; supported are dense float32, bfloat16 and float16");
+        types[i] = code(t);
+        TYPE(types[i] >= 0, who, ": a tensor of type ", name_of(t), "; supported are float32, bfloat16 and float16");
         sizes[i] = t.numel();
         if (out) {
             const Tensor& o = (*out)[i];

@@ -1086,3 +1086,39 @@ def test_gradients_of_a_trace_or_with_a_tangent_are_refused(device):
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match='forward-mode'):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(g, torch.ones_like(g)), retain_graph=True)
         assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
+
+
+class Wrapper(torch.Tensor):
+    """a tensor without memory that says it is on the GPU"""
+    @staticmethod
+    def __new__(cls, like, device='cuda:0'):
+        return torch.Tensor._make_wrapper_subclass(cls, like.shape, dtype=like.dtype, device=device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+def test_tensors_that_wrap_others_are_refused():
+    for call in (lambda t: ops.global_norm([t]), lambda t: ops.clip_global_norm([t], 1.0), lambda t: ops.route(t, 3)):
+        with pytest.raises(TypeError, match='wraps others'):
+            call(Wrapper(torch.ones(4, dtype=torch.float32)))
+    with pytest.raises(TypeError, match='wraps others'):
+        torch.func.vmap(lambda t: ops.global_norm([t]))(torch.ones(2, 3))
+    with pytest.raises(TypeError, match='sparse'):
+        ops.global_norm([torch.ones(3).to_sparse()])
+
+
+@pytest.mark.gpu
+def test_every_operand_that_wraps_others_is_refused(device):
+    """(the checks are the host's: nothing is launched)"""
+    expert, (x, w, b, w2, weights), E = layer_inputs(device, torch.float32)
+    plan = ops.route(expert, E)
+    xs = ops.sort_rows(x, plan)
+    for call in (lambda: ops.route(Wrapper(expert), E), lambda: ops.route(expert, E, Wrapper(expert), 50), lambda: ops.sort_rows(Wrapper(x), plan), lambda: ops.combine_rows(Wrapper(xs), plan),
+                 lambda: ops.combine_rows(xs, plan, Wrapper(weights)), lambda: ops.expert_linear(Wrapper(xs), w, plan, b), lambda: ops.expert_linear(xs, Wrapper(w), plan, b),
+                 lambda: ops.expert_linear(xs, w, plan, Wrapper(b)), lambda: ops.clip_global_norm([x, Wrapper(x)], 1.0), lambda: ops.clip_global_norm([x], 1.0, out=[Wrapper(x)]),
+                 lambda: torch.func.vmap(lambda t: ops.sort_rows(t, plan))(x[None]),
+                 lambda: torch.func.grad(lambda t: ops.sort_rows(t, plan).sum())(x), lambda: ops.sort_rows(x.to_sparse(), plan)):
+        with pytest.raises(TypeError, match='wraps others|sparse'):
+            call()
