@@ -53,8 +53,11 @@ void usable(const char* who, const Tensor& t) {
 }
 void same_device(const char* who, const Tensor& a, const Tensor& b) { VALUE(a.device() == b.device(), who, ": tensors on ", a.device(), " and ", b.device()); }
 
+// a view that stands for the negative of its memory, or for zeros without memory
+bool lazy(const Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+Tensor whole(const Tensor& t) { return lazy(t) ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous(); }
 // a matrix the kernels can read: last dimension contiguous
-Tensor rows_of(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+Tensor rows_of(const Tensor& t) { return !lazy(t) && (t.size(1) <= 1 || t.stride(1) == 1) ? t : whole(t); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // What route() leaves on the device: one int32 tensor with everything in it.
@@ -108,9 +111,9 @@ std::shared_ptr<Plan> route(const Tensor& expert_in, int64_t n_experts, const Ma
         VALUE(n_tokens && *n_tokens >= 0, "route: tokens need n_tokens");
         q->n_tokens = *n_tokens;
         q->listed = true;
-        tokens = tokens_in->contiguous();
+        tokens = whole(*tokens_in);
     }
-    const Tensor expert = expert_in.contiguous();
+    const Tensor expert = whole(expert_in);
     q->n_experts = n_experts;
     q->n_rows = expert.numel();
     q->shape = expert.sizes().vec();
@@ -215,7 +218,7 @@ Tensor combine_rows(const Tensor& ys, const Plan& q, const MaybeTensor& weights_
         VALUE(weights_in->sizes() == at::IntArrayRef(q.shape), "combine_rows: weights ", weights_in->sizes(), " for expert ids ", at::IntArrayRef(q.shape));
         TYPE(weights_in->scalar_type() == at::kFloat || weights_in->scalar_type() == ys.scalar_type(), "combine_rows: weights of type ", name_of(*weights_in), " for rows of type ",
              name_of(ys), "; supported are float32 and the rows' type");
-        weights = weights_in->contiguous();
+        weights = whole(*weights_in);
     }
     if (at::GradMode::is_enabled() && (ys.requires_grad() || wants_grad(weights))) return CombineRows::apply(ys, weights.defined() ? MaybeTensor(weights) : MaybeTensor(), q.buf, &q);
     return combine(ys, q, weights);
@@ -303,11 +306,11 @@ Tensor expert_linear(const Tensor& xs, const Tensor& weight_in, const Plan& q, c
         same_device("expert_linear", xs, *bias_in);
         VALUE(bias_in->dim() == 2 && bias_in->size(0) == weight_in.size(0) && bias_in->size(1) == weight_in.size(1), "expert_linear: bias must be [", weight_in.size(0), ", ", weight_in.size(1),
               "], got ", bias_in->sizes());
-        bias = bias_in->contiguous();
+        bias = whole(*bias_in);
     }
     TYPE(weight_in.scalar_type() == xs.scalar_type() && (!bias.defined() || bias.scalar_type() == xs.scalar_type()), "expert_linear: xs, weight and bias must have one type, got ",
          name_of(xs), ", ", name_of(weight_in), bias.defined() ? text(", ", name_of(bias)) : "");
-    const Tensor weight = weight_in.contiguous();
+    const Tensor weight = whole(weight_in);
     const int64_t act = activation ? CCSP_OPS_SILU : CCSP_OPS_NONE;
     if (at::GradMode::is_enabled() && (xs.requires_grad() || weight.requires_grad() || wants_grad(bias))) return ExpertLinear::apply(xs, weight, bias.defined() ? MaybeTensor(bias) : MaybeTensor(), q.buf, &q, act);
     return linear_forward(rows_of(xs), weight, bias, q, act, nullptr);
@@ -342,12 +345,14 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
             usable(who, o);
             VALUE(o.device() == t.device(), who, ": tensors on ", t.device(), " and ", o.device());
             VALUE(o.scalar_type() == t.scalar_type() && o.sizes() == t.sizes(), who, ": out must hold one tensor of the same type and shape per gradient");
-            VALUE(o.is_contiguous(), who, ": out must be contiguous");
+            VALUE(o.is_contiguous() && !lazy(o), who, ": out must be contiguous");
             to[i] = sizes[i] ? o.data_ptr() : nullptr;
         }
-        if (t.is_contiguous()) from[i] = sizes[i] ? t.data_ptr() : nullptr;
+        VALUE(out || !max_norm || !t._is_zerotensor(), who, ": a tensor without memory cannot be scaled in place");
+        // (in place a negative's memory is scaled like any other)
+        if (t.is_contiguous() && !t._is_zerotensor() && !(out && t.is_neg())) from[i] = sizes[i] ? t.data_ptr() : nullptr;
         else {
-            hold.push_back(t.contiguous());
+            hold.push_back(whole(t));
             from[i] = hold.back().data_ptr();
             if (!out) back.push_back(i);
         }

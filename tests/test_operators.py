@@ -1122,3 +1122,41 @@ def test_every_operand_that_wraps_others_is_refused(device):
                  lambda: torch.func.grad(lambda t: ops.sort_rows(t, plan).sum())(x), lambda: ops.sort_rows(x.to_sparse(), plan)):
         with pytest.raises(TypeError, match='wraps others|sparse'):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('D', [1, 24])
+def test_negative_views_and_zeros_without_memory(device, D):
+    """what torch keeps as a flag on a tensor (the imaginary part of a conjugate; gradients that are zero): the operators see the values"""
+    expert = ids(40, 5, 1, 0.2).reshape(20, 2).to(device)
+    neg, zero = torch._neg_view, torch._efficientzerotensor((20, D), device=device)
+    g = torch.Generator(device=device).manual_seed(0)
+    x, ys, weights = [torch.randn(*s, generator=g, device=device) for s in ((20, D), (40, D), (20, 2))]
+    w, b = torch.randn(5, 3, D, generator=g, device=device), torch.randn(5, 3, generator=g, device=device)
+    assert x.is_contiguous() and neg(x).is_neg() and zero._is_zerotensor()
+    plan = ops.route(expert, 5)
+    assert torch.equal(ops.route(neg(-expert), 5).rows, plan.rows)
+    assert torch.equal(ops.route(expert, 5, neg(-expert), 20).row_token, ops.route(expert, 5, expert, 20).row_token)
+    assert torch.equal(ops.sort_rows(neg(x), plan), ops.sort_rows(-x, plan))
+    assert float(ops.sort_rows(zero, plan).abs().max()) == 0.0
+    assert torch.equal(ops.combine_rows(neg(ys), plan, neg(weights)), ops.combine_rows(-ys, plan, -weights))
+    assert torch.equal(ops.expert_linear(neg(ys), neg(w), plan, neg(b)), ops.expert_linear(-ys, -w, plan, -b))
+    leaves = [t.clone().requires_grad_() for t in (x, ys, weights, w, b)]
+    outs = [ops.sort_rows(leaves[0], plan), ops.combine_rows(leaves[1], plan, leaves[2]), ops.combine_rows(leaves[1], plan), ops.expert_linear(leaves[1], leaves[3], plan, leaves[4], 'silu')]
+    for y, at in zip(outs, ([0], [1, 2], [1], [1, 3, 4])):
+        gy = torch.randn(y.shape, generator=g, device=device)
+        for lazy, plain in ((neg(gy), -gy), (torch._efficientzerotensor(y.shape, device=device), torch.zeros_like(gy))):
+            got, want = [torch.autograd.grad(y, [leaves[i] for i in at], t, retain_graph=True) for t in (lazy, plain)]
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    a, out = torch.ones(4, D, device=device), [torch.empty(4, D, device=device), torch.empty(20, D, device=device)]
+    norm = ops.clip_global_norm([neg(a), zero], 0.5, out=out)
+    assert abs(float(norm) - math.sqrt(4 * D)) < 1e-5 and float(out[1].abs().max()) == 0.0
+    assert float((out[0] + 0.5 / math.sqrt(4 * D)).abs().max()) < 1e-6 and float((a - 1).abs().max()) == 0.0
+    assert abs(float(ops.global_norm([zero, neg(a)])) - math.sqrt(4 * D)) < 1e-5
+    ops.clip_global_norm([neg(a)], 0.5)
+    assert float((a - 0.5 / math.sqrt(4 * D)).abs().max()) < 1e-6
+    with pytest.raises(ValueError, match='without memory'):
+        ops.clip_global_norm([a, zero], 0.1)
+    with pytest.raises(ValueError, match='contiguous'):
+        ops.clip_global_norm([a], 0.1, out=[neg(a.clone())])
+    assert float((a - 0.5 / math.sqrt(4 * D)).abs().max()) < 1e-6      # (refused before anything is written)
