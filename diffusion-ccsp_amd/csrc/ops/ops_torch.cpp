@@ -2,6 +2,7 @@
 // Host code only; the kernels are libccsp_ops.so's.  It exists because a call is short: the smallest operators run 3 us on the GPU, and what
 // a call costs its host -- checks, allocations, the autograd node -- is what a user waits for (in Python: 14 us a call, 50 us with its gradient).
 #include <c10/hip/HIPStream.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -349,6 +350,7 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
             to[i] = sizes[i] ? o.data_ptr() : nullptr;
         }
         VALUE(out || !max_norm || !t._is_zerotensor(), who, ": a tensor without memory cannot be scaled in place");
+        VALUE(out || !max_norm || sizes[i] == 0 || at::has_internal_overlap(t) != at::MemOverlap::Yes, who, ": a tensor whose elements share memory (an expanded one) cannot be scaled in place");
         // (in place a negative's memory is scaled like any other)
         if (t.is_contiguous() && !t._is_zerotensor() && !(out && t.is_neg())) from[i] = sizes[i] ? t.data_ptr() : nullptr;
         else {

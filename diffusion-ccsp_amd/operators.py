@@ -59,7 +59,7 @@ def global_norm(tensors):
 
 def clip_global_norm(grads, max_norm, out=None):
     """Scales the tensors by min(1, max_norm / (norm + 1e-6)), norm their global norm before scaling, which is returned (a float32 scalar on the device;
-    nothing waits for it).  In place, or into `out`: contiguous tensors of the same types and shapes, each the same memory as its gradient or disjoint from
+    nothing waits for it).  In place (gradients that are not expanded), or into `out`: contiguous tensors of the same types and shapes, each the same memory as its gradient or disjoint from
     all (checked).  Types may differ from tensor to tensor.  A norm that is not finite gives what the formula gives: factor 0 for infinity, NaN for NaN."""
     return _ops.torch_ops().clip('clip_global_norm', list(grads), float(max_norm), out if out is None else list(out))
 

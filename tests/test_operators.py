@@ -1160,3 +1160,21 @@ def test_negative_views_and_zeros_without_memory(device, D):
     with pytest.raises(ValueError, match='contiguous'):
         ops.clip_global_norm([a], 0.1, out=[neg(a.clone())])
     assert float((a - 0.5 / math.sqrt(4 * D)).abs().max()) < 1e-6      # (refused before anything is written)
+
+
+@pytest.mark.gpu
+def test_expanded_gradients_are_refused_in_place_before_anything_is_scaled(device):
+    a, e = torch.ones(4, device=device), torch.ones(1, device=device).expand(5)
+    for grads in ([a, e], [e, a], [a, torch.ones(2, 1, device=device).expand(2, 3)]):
+        with pytest.raises(ValueError, match='share memory'):
+            ops.clip_global_norm(grads, 0.5)
+    p = torch.nn.Parameter(torch.zeros(5, device=device))
+    p.grad = e
+    with pytest.raises(ValueError, match='share memory'):
+        ops.clip_grad_norm_([p], 0.5)
+    assert float((a - 1).abs().max()) == 0.0 and float(e[0]) == 1.0
+    none = torch.ones(1, device=device).expand(0)
+    out = [torch.empty(4, device=device), torch.empty(5, device=device), torch.empty(0, device=device)]
+    assert float(ops.clip_global_norm([a, e, none], 1.5, out=out)) == 3.0 == float(ops.global_norm([a, e]))      # (every element counts)
+    assert float((out[0] - 0.5).abs().max()) < 1e-6 and float((out[1] - 0.5).abs().max()) < 1e-6
+    assert float(ops.clip_global_norm([a, none], 1.0)) == 2.0 and float((a - 0.5).abs().max()) < 1e-6
