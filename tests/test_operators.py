@@ -1178,3 +1178,50 @@ def test_expanded_gradients_are_refused_in_place_before_anything_is_scaled(devic
     assert float(ops.clip_global_norm([a, e, none], 1.5, out=out)) == 3.0 == float(ops.global_norm([a, e]))      # (every element counts)
     assert float((out[0] - 0.5).abs().max()) < 1e-6 and float((out[1] - 0.5).abs().max()) < 1e-6
     assert float(ops.clip_global_norm([a, none], 1.0)) == 2.0 and float((a - 0.5).abs().max()) < 1e-6
+
+
+# ---- the training command ------------------------------------------------------------------------------------------------
+
+def check_absent_types(monkeypatch, dev, operators_on):
+    monkeypatch.setenv('TRAIN_DEVICE', dev)
+    monkeypatch.setenv('TRAIN_HIDDEN', '64')
+    monkeypatch.setenv('TRAIN_OPERATORS', operators_on)
+    monkeypatch.syspath_prepend(os.path.join(ROOT, 'tools'))
+    monkeypatch.delitem(sys.modules, 'train_gpu', raising=False)
+    import train_gpu as tg
+    assert tg.USE_OPERATORS == (operators_on == '1')
+    rng = np.random.default_rng(4)
+    ws = [worlds.sample_qualitative_world(rng, int(rng.integers(2, 9))) for _ in range(24)]
+    batch = worlds.collate([worlds.encode_qualitative(w['nodes'], w['constraints']) for w in ws])
+    kinds = np.asarray(batch.edge_attr).reshape(-1).astype(int)
+    gone = int(np.bincount(kinds[kinds >= 0]).argmax())           # a type that the first batch has
+    torch.manual_seed(1)
+    net = tg.Denoiser().to(dev)
+    opt = torch.optim.Adam(net.parameters(), lr=5e-4)
+    sa, sb = tg.schedule_tables()
+    noise, t = torch.randn(batch.x.shape[0], 4, device=dev), torch.tensor([300], device=dev)
+    tg.train_step(net, opt, tg.to_dev(batch), t, noise, sa, sb)
+    before = {n: p.detach().clone() for n, p in net.named_parameters()}
+    moment = opt.state[net.mlps[gone][0].weight]['exp_avg'].clone()
+    assert float(moment.abs().max()) > 0.0
+    keep = kinds != gone
+    batch.edge_attr, batch.edge_index = batch.edge_attr[keep], batch.edge_index[:, keep]
+    b = tg.to_dev(batch)
+    assert gone in b['absent']
+    assert bool(torch.isfinite(tg.train_step(net, opt, b, t, noise, sa, sb)))
+    for i, mlp in enumerate(net.mlps):
+        for n, p in mlp.named_parameters():
+            assert torch.equal(p.detach(), before['mlps.%d.%s' % (i, n)]) == (i in b['absent']), (i, n)
+    assert torch.equal(opt.state[net.mlps[gone][0].weight]['exp_avg'], moment)
+    monkeypatch.delitem(sys.modules, 'train_gpu', raising=False)
+
+
+def test_a_type_without_edges_is_not_trained(monkeypatch):
+    """its weights and moments stay as they are, as where its MLP is not called at all"""
+    check_absent_types(monkeypatch, 'cpu', '0')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('operators_on', ['0', '1'])
+def test_a_type_without_edges_is_not_trained_on_the_gpu(device, monkeypatch, operators_on):
+    check_absent_types(monkeypatch, 'cuda:0', operators_on)

@@ -106,6 +106,7 @@ def to_dev(batch):
     for i in range(C):
         d['ea'].append(e0[bounds[i]:bounds[i + 1]])
         d['eb'].append(e1[bounds[i]:bounds[i + 1]])
+    d['absent'] = [i for i in range(C) if bounds[i] == bounds[i + 1]]
     cnt = np.bincount(ei.reshape(-1), minlength=batch.x.shape[0]).astype(np.float32)
     d['cnt'] = torch.from_numpy(cnt).to(dev, non_blocking=True)
     d['nodes'] = d['edges'] = None
@@ -136,6 +137,20 @@ def loss_on(net, b, t, noise, sa, sb):
     xt = sa[t] * x0 + sb[t] * noise
     xt = torch.where(b['mask'][:, None], x0, xt)
     return F.mse_loss(net(xt, b, t), noise)
+
+
+def train_step(net, opt, b, t, noise, sa, sb):
+    loss = loss_on(net, b, t, noise, sa, sb)
+    opt.zero_grad(set_to_none=True)
+    loss.backward()
+    # a type without edges in the batch has no gradient (the operators' is zero, which Adam would answer with a step of its moments)
+    for i in b['absent']:
+        for p in net.mlps[i].parameters():
+            p.grad = None
+    if CLIP > 0:
+        operators.clip_grad_norm_(net.parameters(), CLIP) if USE_OPERATORS else torch.nn.utils.clip_grad_norm_(net.parameters(), CLIP)
+    opt.step()
+    return loss
 
 
 def main():
@@ -174,12 +189,7 @@ def main():
             batches = epoch_batches()
         b = batches[step % len(batches)]
         t = torch.randint(0, T, (1,), device=dev)
-        loss = loss_on(net, b, t, torch.randn_like(b['x'][:, dims[-1][1]:dims[-1][2]]), sa, sb)
-        opt.zero_grad(set_to_none=True)
-        loss.backward()
-        if CLIP > 0:
-            operators.clip_grad_norm_(net.parameters(), CLIP) if USE_OPERATORS else torch.nn.utils.clip_grad_norm_(net.parameters(), CLIP)
-        opt.step()
+        loss = train_step(net, opt, b, t, torch.randn_like(b['x'][:, dims[-1][1]:dims[-1][2]]), sa, sb)
         run = 0.99 * run + 0.01 * loss.item() if step % 50 == 0 and step else run
         if step in ckpts:
             save(net, out_path.replace('.npz', '_%dk.npz' % (step // 1000)), step)
