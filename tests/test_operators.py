@@ -1225,3 +1225,87 @@ def test_a_type_without_edges_is_not_trained(monkeypatch):
 @pytest.mark.parametrize('operators_on', ['0', '1'])
 def test_a_type_without_edges_is_not_trained_on_the_gpu(device, monkeypatch, operators_on):
     check_absent_types(monkeypatch, 'cuda:0', operators_on)
+
+# ---- every tile of the products ------------------------------------------------------------------------------------------
+
+def most_tiles(R, E, l):
+    return (R >> l) + min(R, E + 1)
+
+
+def prod_tile(weight, R, E, M, N):
+    """the rule of csrc/ops/ops_linear.h prod_tile for 16 bits, restated"""
+    tiles = lambda l: (E * -(-M >> l) if weight else most_tiles(R, E, l)) * -(-N >> l)      # noqa: E731
+    big = tiles(8)
+    if (big >= 256 and R >= 1024 * E) if weight else (big >= 1024 or (big >= 512 and R >= 1024 * E)):
+        return 256
+    return 128 if tiles(7) >= 512 else 64
+
+
+def seg_log2(R, E, M, N):
+    """the rule of seg_log2_for for 16 bits, restated; 31: uncut"""
+    tile = prod_tile(True, R, E, M, N)
+    tiles = -(-M // tile) * -(-N // tile)
+    if tile == 256 or tiles >= 128:
+        return 31
+    l = 10
+    while l < 30 and (2 << l) <= R * tiles // 1024:
+        l += 1
+    return 31 if 1 << l >= R else l
+
+
+# counts, tail, inputs, outputs, tiles of the forward, the input gradient and the weight gradient, the weight gradient's segment
+TILES = [([3000, 1024, 0, 1025, 951], 3, 1240, 1288, 128, 128, 128, 10),             # an expert longer than a segment, at its border, without rows
+         ([3000, 1024, 0, 1025, 951], 3, 1237, 1285, 128, 128, 128, 10),             # results without whole pieces
+         ([900, 0, 3, 1, 50], 0, 1240, 1288, 64, 64, 128, 31),                       # few rows: uncut
+         ([4000, 1, 0, 3000], 5, 1400, 1416, 128, 128, 128, 31),                     # enough tiles: uncut
+         ([4000, 1, 0, 3000], 5, 1401, 1419, 128, 128, 128, 31),
+         ([9000, 1, 0, 3999], 2, 264, 4099, 256, 64, 64, 31),                        # 256 x 256 without whole pieces, forward
+         ([9000, 1, 0, 3999], 2, 4099, 264, 64, 256, 64, 31),                        # and input gradient
+         ([9000, 1, 0, 3999], 0, 2049, 4099, 256, 128, 256, 31)]                     # and weight gradient
+
+
+@pytest.mark.parametrize('case', TILES, ids=str)
+def test_the_cases_below_reach_the_tiles_that_they_name(case):
+    """by the rules restated above; the rules' own lines and, for the segments, the workspace say that they are still the library's"""
+    counts, tail, I, O, forward, back_input, back_weight, seg = case
+    R, E = sum(counts) + tail, len(counts)
+    assert prod_tile(False, R, E, O, O) == forward and prod_tile(False, R, E, O, I) == back_input
+    assert prod_tile(True, R, E, O, I) == back_weight and seg_log2(R, E, O, I) == seg
+    text = open(os.path.join(ROOT, 'diffusion-ccsp_amd', 'csrc', 'ops', 'ops_linear.h')).read()
+    for line in ('inline long most_tiles(long R, long E, int l) { const long g = R < E + 1 ? R : E + 1; return (R >> l) + g; }',
+                 'return (weight ? E * cdiv(M, 1l << l) : most_tiles(R, E, l)) * cdiv(N, 1l << l);',
+                 'if (weight ? big >= 256 && R >= 1024 * E : big >= 1024 || (big >= 512 && R >= 1024 * E)) return TILE_256;',
+                 'return prod_tiles(weight, R, E, M, N, 7) >= 512 ? TILE_128 : TILE_64;',
+                 'prod_tile<T>(PROD == PROD_WEIGHT, p.R, p.E, out, PROD == PROD_FORWARD ? out : inp)'):
+        assert line in text, line
+    padded = lambda n: -(-n // 8) * 8      # noqa: E731
+    need = sum(-(-R * padded(n) * 2 // 256) * 256 for n in (I, O) if n % 8)
+    if seg != 31:
+        need += 2 * ((R >> seg) + 1) * ((O * I + O + 3) // 4 * 4) * 4
+    assert _ops.lib().ccsp_ops_linear_workspace(2, 1, E, R, I, O, 64, O, 64, I) == need
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('case', TILES, ids=str)
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('act', [None, 'silu'])
+def test_expert_linear_in_every_tile_with_gradients(device, case, dtype, act):
+    counts, tail, I, O = case[:4]
+    check_linear(device, counts, tail, I, O, DTYPES[dtype], act, True, where=device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('case', TILES, ids=str)
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+def test_the_bias_gradient_alone_in_every_tile(device, case, dtype):
+    """the bits that it has beside the weights' gradient, where a tile of 128 x 128 makes it too"""
+    counts, tail, I, O = case[:4]
+    expert = torch.cat([torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts)), torch.full((tail,), -1)]).to(device)
+    plan = ops.route(expert, len(counts))
+    g = torch.Generator(device=device).manual_seed(8)
+    xs, w, bias, gy = [torch.randn(*s, generator=g, device=device).to(DTYPES[dtype]) for s in ((len(expert), I), (len(counts), O, I), (len(counts), O), (len(expert), O))]
+    bias.requires_grad_()
+    alone, = torch.autograd.grad(ops.expert_linear(xs, w, plan, bias), bias, gy)
+    w.requires_grad_()
+    beside = torch.autograd.grad(ops.expert_linear(xs, w, plan, bias), (w, bias), gy)[1]
+    assert torch.equal(alone, beside)
