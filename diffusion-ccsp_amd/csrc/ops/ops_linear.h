@@ -100,7 +100,7 @@ __device__ __forceinline__ f32x4 mfma16(Vec8<fp16>::t a, Vec8<fp16>::t b, f32x4 
 // ------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void lds_dma16(u32x4 rsrc, unsigned int offset, unsigned int lds) {
     // (five wait states between a vector instruction's scalar result, as the descriptor may be one, and the load: the compiler does not see the load)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory", "m0");
 }
 constexpr unsigned int DMA_OUT = 0x80000000u;                    // an offset past every buffer
 
