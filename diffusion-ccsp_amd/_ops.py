@@ -7,6 +7,7 @@ import importlib.util
 import os
 import shutil
 import subprocess
+import threading
 
 from ._lib import CSRC, CcspError
 
@@ -66,13 +67,30 @@ def _ensure():
 
 
 _lib = _torch = None
+_loading = threading.RLock()      # the first calls may come from several threads
 
 
 def lib():
     """the C ABI (include/ccsp_ops.h) through ctypes"""
     global _lib
-    if _lib is not None:
-        return _lib
+    if _lib is None:
+        with _loading:
+            if _lib is None:
+                _lib = _load_lib()
+    return _lib
+
+
+def torch_ops():
+    """the operators on torch tensors (csrc/ops/ops_torch.cpp)"""
+    global _torch
+    if _torch is None:
+        with _loading:
+            if _torch is None:
+                _torch = _load_torch()
+    return _torch
+
+
+def _load_lib():
     _ensure()
     try:
         L = C.CDLL(OPS_SO)
@@ -97,15 +115,10 @@ def lib():
     L.ccsp_ops_norm_workspace.argtypes = [i32, vp]
     L.ccsp_ops_norm_workspace.restype = i64
     L.ccsp_ops_clip_norm.argtypes = [i32, vp, vp, vp, vp, C.c_double, vp, vp, vp, i64, vp]
-    _lib = L
     return L
 
 
-def torch_ops():
-    """the operators on torch tensors (csrc/ops/ops_torch.cpp)"""
-    global _torch
-    if _torch is not None:
-        return _torch
+def _load_torch():
     _ensure()
     import torch  # noqa: F401  (its libraries come first)
     try:
@@ -116,10 +129,4 @@ def torch_ops():
         raise CcspError('cannot load %s: %s (the HIP extension is required)' % (TORCH_SO, e))
     _check_version(TORCH_SO, m.version())
     m.set_error(CcspError)
-    _torch = m
     return m
-
-
-def check(rc):
-    if rc != 0:
-        raise CcspError(lib().ccsp_ops_last_error().decode())

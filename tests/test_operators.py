@@ -1309,3 +1309,40 @@ def test_the_bias_gradient_alone_in_every_tile(device, case, dtype):
     w.requires_grad_()
     beside = torch.autograd.grad(ops.expert_linear(xs, w, plan, bias), (w, bias), gy)[1]
     assert torch.equal(alone, beside)
+
+
+# ---- loading -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('which', ['lib', 'torch_ops'])
+def test_first_calls_from_several_threads_load_once(monkeypatch, which):
+    """each loader waits until the others had time to come in too"""
+    import time
+    loads, name = [], {'lib': '_lib', 'torch_ops': '_torch'}[which]
+
+    def ensure():
+        loads.append(threading.get_ident())
+        time.sleep(0.2)
+    monkeypatch.setattr(_ops, '_ensure', ensure)
+    monkeypatch.setattr(_ops, name, None)
+    if which == 'torch_ops':
+        class Loader:
+            def __init__(self, *args):
+                pass
+
+            def create_module(self, spec):
+                return None
+
+            def exec_module(self, m):
+                m.version, m.set_error = (lambda: 1000 * _ops.OPS_ABI_MAJOR), (lambda e: None)
+        monkeypatch.setattr(_ops.importlib.machinery, 'ExtensionFileLoader', Loader)
+    got, gate = [], threading.Barrier(4)
+
+    def first():
+        gate.wait()
+        got.append(getattr(_ops, which)())
+    threads = [threading.Thread(target=first) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(loads) == 1 and len(got) == 4 and all(g is got[0] for g in got)
