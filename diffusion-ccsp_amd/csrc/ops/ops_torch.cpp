@@ -40,11 +40,14 @@ struct On {
     explicit On(const Tensor& t) : guard(t.device()), stream((void*)c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-// what every tensor of a call has to be
-void usable(const char* who, const Tensor& t) {
-    // (a trace records torch's own operations: of a kernel, nothing but the memory that its result goes to)
+// (a trace records torch's own operations: of a kernel, nothing but the memory that its result goes to)
+void not_recorded(const char* who) {
     if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch))
         throw OpsError(text(who, ": cannot be recorded by torch.jit.trace or make_fx; it may be captured into a graph of the GPU's"));
+}
+
+// what every tensor of a call has to be
+void usable(const char* who, const Tensor& t) {
     // (a tangent would be lost without a word: the kernels read the values alone)
     if (t._fw_grad(0).defined()) throw OpsError(text(who, ": forward-mode derivatives are not supported; gradients come through torch.autograd in reverse"));
     // (a wrapper -- a distributed or quantised tensor, one inside torch.func's transforms -- has no memory of its own, or memory that means something else)
@@ -93,6 +96,7 @@ struct Plan {
 };
 
 std::shared_ptr<Plan> route(const Tensor& expert_in, int64_t n_experts, const MaybeTensor& tokens_in, c10::optional<int64_t> n_tokens) {
+    not_recorded("route");
     usable("route", expert_in);
     TYPE(expert_in.scalar_type() == at::kInt || expert_in.scalar_type() == at::kLong, "route: expert ids must be int32 or int64, got ", name_of(expert_in));
     VALUE(n_experts >= 1 && n_experts <= CCSP_OPS_MAX_EXPERTS, "route: ", n_experts, " experts, supported are 1 to ", CCSP_OPS_MAX_EXPERTS);
@@ -162,6 +166,7 @@ struct SortRows : torch::autograd::Function<SortRows> {
     static variable_list backward(AutogradContext* c, variable_list g) {
         const bool more = at::GradMode::is_enabled();
         at::NoGradGuard no;
+        not_recorded("sort_rows");
         usable("sort_rows", g[0]);
         const Plan q = Plan::load(c, c->get_saved_variables()[0]);
         return first_order("sort_rows", more, {combine(g[0], q, Tensor()), Tensor(), Tensor()});
@@ -179,6 +184,7 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
     static variable_list backward(AutogradContext* c, variable_list grads) {
         const bool more = at::GradMode::is_enabled();
         at::NoGradGuard no;
+        not_recorded("combine_rows");
         usable("combine_rows", grads[0]);
         const auto saved = c->get_saved_variables();
         const Plan q = Plan::load(c, saved[0]);
@@ -201,6 +207,7 @@ void float_rows(const char* who, const char* name, const Tensor& t, int64_t n, c
 }
 
 Tensor sort_rows(const Tensor& x, const Plan& q) {
+    not_recorded("sort_rows");
     usable("sort_rows", x);
     same_device("sort_rows", x, q.buf);
     float_rows("sort_rows", "x", x, q.n_tokens, "one row per token");
@@ -209,6 +216,7 @@ Tensor sort_rows(const Tensor& x, const Plan& q) {
 }
 
 Tensor combine_rows(const Tensor& ys, const Plan& q, const MaybeTensor& weights_in) {
+    not_recorded("combine_rows");
     usable("combine_rows", ys);
     same_device("combine_rows", ys, q.buf);
     float_rows("combine_rows", "ys", ys, q.n_rows, "one row per assignment");
@@ -261,6 +269,7 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
     static variable_list backward(AutogradContext* c, variable_list grads) {
         const bool more = at::GradMode::is_enabled();
         at::NoGradGuard no;
+        not_recorded("expert_linear");
         usable("expert_linear", grads[0]);
         const auto saved = c->get_saved_variables();
         const Plan q = Plan::load(c, saved[0]);
@@ -292,6 +301,7 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
 };
 
 Tensor expert_linear(const Tensor& xs, const Tensor& weight_in, const Plan& q, const MaybeTensor& bias_in, const c10::optional<std::string>& activation) {
+    not_recorded("expert_linear");
     usable("expert_linear", xs);
     usable("expert_linear", weight_in);
     same_device("expert_linear", xs, q.buf);
@@ -331,6 +341,7 @@ Tensor clip(const std::string& name, const std::vector<Tensor>& src, c10::option
     std::vector<void*> to(n);
     std::vector<int64_t> sizes(n);
     std::vector<int32_t> types(n);
+    not_recorded(who);
     usable(who, src[0]);
     On on(src[0]);
     at::NoGradGuard no;

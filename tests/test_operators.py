@@ -1346,3 +1346,26 @@ def test_first_calls_from_several_threads_load_once(monkeypatch, which):
     for t in threads:
         t.join()
     assert len(loads) == 1 and len(got) == 4 and all(g is got[0] for g in got)
+
+# ---- streams -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_a_plan_recorded_on_another_stream_outlives_its_name(device):
+    """the owner of a plan that another stream still reads records it there, as any tensor: its memory is not given away before"""
+    expert = ids(60000, 20, 3, 0.1).to(device)
+    x = torch.randn(60000, 64, device=device)
+    want = ops.sort_rows(x, ops.route(expert, 20))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    plan = ops.route(expert, 20)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            got = ops.sort_rows(x, plan)
+    size = plan.offsets.untyped_storage().nbytes()
+    plan.offsets.record_stream(s)
+    del plan
+    for _ in range(4):                                            # (on the plan's own stream, while the other may still be at work)
+        torch.full((size // 4,), -1, dtype=torch.int32, device=device)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
