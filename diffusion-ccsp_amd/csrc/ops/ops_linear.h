@@ -463,7 +463,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_product(ProdArgs p, int til
         // 16 (TN / WN) / 8 bytes instead of sixteen rows' 32: 65536 rows, 16 experts 2048 -> 4096: 1220 -> 1080 us.  Where the last-level cache cannot
         // hold operands and result together, results are written past it and leave it to the operands, which other tiles and the next products read again: 8192 rows, 32 experts
         // 2048 -> 1408 with gradients (184 MB of weights) 286 -> 258 us, of which only the weight gradient past it 277; the weight gradient of 64 experts 2048 -> 1408 of
-        // 2048 rows 117 -> 98 us.  Where all fits, a result is read from the cache next.
+        // 2048 rows 117 -> 98 us.  Where all fits, a result is read from the cache next; a combine_rows that reads one from behind the cache is no slower for it (8192 rows,
+        // 32 experts 2048 -> 1408, product and combine: 77 us either way; 4096 rows, 64 experts 2048 -> 1024: 61 and 62).
         if (p.pieces == 8 && !part) {
             constexpr int PM = TM / WM, PN = TN / WN, CH = PN / 8;         // the wave's part, 16-byte pieces of its row
             T* const own = reinterpret_cast<T*>(lds) + wave * PM * PN;
@@ -616,7 +617,9 @@ __global__ __launch_bounds__(256) void k_pad_rows(PadJob j0, PadJob j1) {
 }
 
 // ---- around the products -------------------------------------------------------------------------------------------------
-// dz = dy silu'(z) over the active rows (z as it was stored: its rounding moves the slope by less than dz's own rounding does)
+// dz = dy silu'(z) over the active rows, rounded to the type that the matrix pipe takes it in.  z is as it was stored: in 16 bits its rounding moves the slope by up to
+// |silu''| u |z| <= u |z| / 2, which for most z below -0.6 is more than dz's own rounding (near the slope's zero at -1.28 by any factor).  The alternative is z in 32 bits, 2 bytes a value
+// more to write and read.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_silu_back(const int* __restrict__ active, int width, const T* __restrict__ dy, long dy_stride, const T* __restrict__ z, T* __restrict__ dz) {
     typedef typename LooseOf<T, V>::type VT;

@@ -138,7 +138,7 @@ __device__ __forceinline__ void clip_chunk(const T* p, T* o, long n, float c) {
 
 __global__ __launch_bounds__(256) void k_norm_clip(NormTable t, int blocks, const float* scale) {
     const float c = scale[0];
-    const int b = blocks - 1 - blockIdx.x;                       // from the end: what the norm read last is still in the last-level cache
+    const int b = blocks - 1 - blockIdx.x;                       // a table from its end: with one table, what the norm read last is still in the last-level cache
     const int i = norm_tensor(t, b);
     if (c == 1.0f && t.in[i] == t.out[i]) return;                // g x 1 in place
     const long at = (long)(b - t.first[i]) * t.chunk;
@@ -148,7 +148,8 @@ __global__ __launch_bounds__(256) void k_norm_clip(NormTable t, int blocks, cons
     else clip_chunk(static_cast<const fp16*>(t.in[i]) + at, static_cast<fp16*>(t.out[i]) + at, n, c);
 }
 
-// hands tables of at most NORM_TENSORS tensors that have elements to f(table, blocks, blocks before it), first to last or last to first
+// hands tables of at most NORM_TENSORS tensors that have elements to f(table, blocks, blocks before it), first to last.  (With several tables clip starts on the first, which
+// the norm read longest ago.)
 template <typename F>
 int norm_tables(int count, const void* const* in, void* const* out, const int64_t* n, const int32_t* type, F&& f) {
     const long chunk = norm_chunk_for(count, n);

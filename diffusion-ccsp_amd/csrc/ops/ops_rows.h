@@ -13,13 +13,16 @@
 // and its row comes out of a cache instead of once per expert over the fabric, while the rows written are scattered.  Worth it for rows of ROWS_BY_TOKEN bytes
 // and more (4096 tokens x 4, 4096 in bf16: gather 39 -> 28 us, back 62 -> 57); shorter ones would scatter pieces of lines.
 constexpr int ROWS_BY_TOKEN = 512;
-// Results that the last-level cache (256 MB) cannot hold anyway are written past it, which leaves it to the rows that are read again: 32768 tokens x 8, 2048 in
-// bf16 (1 GB): gather 317 -> 194 us, 6.2 TB/s; 65536 x 2, 1024 (268 MB): 79 -> 60; but 4096 x 4, 4096 (134 MB): 27.5 -> 28.8.
-// (back: 449 -> 430 and 129 -> 124 us.)
+// Results that the last-level cache (256 MB) cannot hold anyway are written past it, which leaves it to the tokens' rows where those are in it: 32768 tokens x 8, 2048 in
+// bf16 (1 GB from 134 MB), written into the cache against past it: gather in a loop 317 us against 197, behind combine's result 320 against 202, behind back's 305 against 229;
+// but where another GB was written or read before it there is nothing to keep: 323 against 330, 308 against 316, and a training step over such rows has 293.  In
+// loops: 65536 x 2, 1024 (268 MB) 79 against 60; but 4096 x 4, 4096 (134 MB) 27.5 against 28.8.  (back: 449 against 430 and 129 against 124.)
 constexpr long ROWS_PAST_CACHE = 192l << 20;
 // combine reads each of its rows once; past the cache they leave it to what the next kernels read, unless they are few enough to be read from it again by the
 // gradient.  A pass of gather, combine, back, combine in 16 bits, kept in the cache against past it: 4099 tokens x 3, 1024 (25 MB) 37 us against 40; 8192 x 4, 1024 (67 MB)
-// 70 against 75; but 20264 x 2, 512 in 32 bits (83 MB) 106 against 104; 16384 x 4, 1024 (134 MB) 155 against 145; 32768 x 4, 1024 (268 MB) 317 against 279.
+// 71 against 74; 16384 x 4, 1024 (134 MB) 155 against 144; 32768 x 4, 1024 (268 MB) 317 against 279.  Between 75 and 120 MB it goes by what else the pass holds:
+// 8192 x 5 (84 MB) 85 against 92, 8192 x 6 (101 MB) 98 against 104, but 12288 x 4 (101 MB) 113 against 104, 8192 x 7 (117 MB) 127 against 119; in 32 bits 10000 x 2, 1024
+// (82 MB) 104 against 100; 40528 rows of 2304 tokens, 512 (83 MB) 89 against 97, but 146 against 135 where combine's rows are not what gather wrote, as behind a product.
 constexpr long ROWS_READ_ONCE = 72l << 20;
 
 struct RowOrder {

@@ -10,10 +10,16 @@
 The denoiser is such a layer: an edge of type e sends its two nodes through the MLP of type e and adds the results onto them with the weight
 1 / sqrt(degree) (networks/denoise_fn.py:313-389, :508-523); tools/train_gpu.py trains it with these operators.
 
-Tensors live on one GPU, rows in float32, bfloat16 or float16; sums are held in 32 bits and rounded once.  Work goes to the current stream of the tensors'
-device, nothing waits for it, and a call may be captured into a graph (a backward pass through torch.autograd.grad, as nothing may be left to do on the
-leaves' own stream).  The gradients of sort_rows, combine_rows and expert_linear come through torch.autograd (first order, in reverse: forward-mode derivatives raise).  torch.jit.trace and make_fx record torch's own
-operations only: an operator raises under them.  Every operator gives the same bits for the same inputs.
+Tensors live on one GPU, rows in float32, bfloat16 or float16; sums are held in 32 bits and each result is rounded once.  expert_linear with an activation
+keeps two values between its forward and its backward in the rows' type as well: the pre-activation, and the gradient of it that the matrix instructions take (in
+float16 one beyond 65504 is infinite, like any result).
+
+Work goes to the current stream of the tensors' device and nothing waits for it.  A plan or tensor that another stream uses is recorded there by its owner, as
+everywhere in torch (plan.offsets.record_stream).  A call may be captured into a graph (a backward pass through torch.autograd.grad, as nothing may be left to do
+on the leaves' own stream).  torch.jit.trace and make_fx record torch's own operations only: an operator raises under them, and for tensors that wrap others.
+
+The gradients of sort_rows, combine_rows and expert_linear come through torch.autograd, first order and in reverse (forward-mode derivatives raise).  Every
+operator gives the same bits for the same inputs.
 """
 import torch
 

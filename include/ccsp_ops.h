@@ -76,7 +76,7 @@ int64_t ccsp_ops_linear_workspace(int32_t product, int32_t type, int32_t n_exper
                                   int64_t b_stride);
 int ccsp_ops_linear(int32_t type, int32_t n_experts, int64_t n_rows, int64_t inp, int64_t out, const int32_t* offsets, const void* x, int64_t x_stride, const void* weight,
                     const void* bias, int32_t activation, void* y, void* z, void* workspace, int64_t workspace_bytes, void* stream);
-/* dz = dy * silu'(z) in the active rows; the rows behind are not written. */
+/* dz = dy * silu'(z) in the active rows, rounded to the type; the rows behind are not written. */
 int ccsp_ops_linear_silu_back(int32_t type, int32_t n_experts, int64_t n_rows, int64_t out, const int32_t* offsets, const void* dy, int64_t dy_stride, const void* z, void* dz,
                               void* stream);
 /* dx = dz weight[e] [n_rows, inp], zeros behind the last active row. */

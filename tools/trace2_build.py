@@ -1,4 +1,4 @@
-"""Builds tools/abl_trace2.so: the product kernels with -DCCSP_TRACE2 (ccsp_hip.hip: per-workgroup phase stamps of k_rowgemm_h2 through LDS, the
+"""Builds tools/abl_trace2.so: the product kernels with -DCCSP_TRACE2 (ccsp_trace.h: per-workgroup phase stamps of k_rowgemm_h2, stored by lane 0, the
 hardware slot of every workgroup), at the product residency.  usage: python tools/trace2_build.py && gpurun -- python tools/trace2_run.py 256"""
 import os
 import sys
