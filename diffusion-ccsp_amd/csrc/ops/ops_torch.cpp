@@ -50,9 +50,10 @@ void not_recorded(const char* who) {
 void usable(const char* who, const Tensor& t) {
     // (a tangent would be lost without a word: the kernels read the values alone)
     if (t._fw_grad(0).defined()) throw OpsError(text(who, ": forward-mode derivatives are not supported; gradients come through torch.autograd in reverse"));
-    // (a wrapper -- a distributed or quantised tensor, one inside torch.func's transforms -- has no memory of its own, or memory that means something else)
+    // (a wrapper -- a distributed or quantised tensor, one inside torch.func's transforms -- has no memory of its own)
     TYPE(t.layout() == at::kStrided, who, ": a tensor that is sparse or blocked; supported are dense ones");
-    TYPE(!t.unsafeGetTensorImpl()->is_python_dispatch() && t.has_storage(), who, ": a tensor that wraps others (a subclass with its own dispatch, a transform's); supported are plain ones");
+    TYPE(t.has_storage() && (!t.unsafeGetTensorImpl()->is_python_dispatch() || t.unsafeGetTensorImpl()->unsafe_storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks().get()), who,
+         ": a tensor that wraps others (a subclass without memory, a transform's); supported are plain ones");
     if (!t.is_cuda()) throw OpsError(text(who, ": tensors must be on a GPU (got ", t.device(), "); there is no CPU fallback"));
 }
 void same_device(const char* who, const Tensor& a, const Tensor& b) { VALUE(a.device() == b.device(), who, ": tensors on ", a.device(), " and ", b.device()); }

@@ -8,6 +8,7 @@
  * Conventions
  *  - every array pointer is a DEVICE pointer owned by the caller unless the parameter is documented "host"; rows are contiguous in their
  *    last dimension, *_stride is the distance of two rows in ELEMENTS; an element pointer is aligned to its element, nothing more;
+ *  - results and workspaces overlap no operand and not each other (clip_norm: as it says); workspaces are aligned to 16 bytes;
  *  - every call enqueues its work on `stream` (hipStream_t as void*; NULL = the default stream) of the CURRENT device and returns: nothing here
  *    allocates, synchronises or copies to the host, so every call may be captured into a graph;
  *  - return value 0 = ok, non-zero = error; ccsp_ops_last_error() gives the thread-local message; no exception crosses the boundary;

@@ -1369,3 +1369,32 @@ def test_a_plan_recorded_on_another_stream_outlives_its_name(device):
         torch.full((size // 4,), -1, dtype=torch.int32, device=device)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+# ---- subclasses with memory ----------------------------------------------------------------------------------------------
+
+class Counted(torch.Tensor):
+    """a subclass with its own dispatch whose memory is its values"""
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        strip = lambda t: t.as_subclass(torch.Tensor) if isinstance(t, Counted) else t      # noqa: E731
+        return func(*[strip(a) for a in args], **(kwargs or {}))
+
+
+@pytest.mark.gpu
+def test_a_subclass_with_memory_is_read_as_its_values(device):
+    expert, (x, w, b, w2, weights), E = layer_inputs(device, torch.float32)
+    plan = ops.route(expert, E)
+    sub = torch.Tensor._make_subclass(Counted, x)
+    assert type(sub) is Counted and sub.data_ptr() == x.data_ptr()
+    assert torch.equal(ops.sort_rows(sub, plan), ops.sort_rows(x, plan))
+    assert float(ops.global_norm([sub])) == float(ops.global_norm([x]))
+
+
+def test_fake_tensors_are_refused():
+    """tensors that say they are on the GPU and have no memory there"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        t = torch.empty(4, device='cuda:0')
+    with pytest.raises(TypeError, match='wraps others'):
+        ops.global_norm([t])
