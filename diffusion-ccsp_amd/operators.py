@@ -15,8 +15,9 @@ keeps two values between its forward and its backward in the rows' type as well:
 float16 one beyond 65504 is infinite, like any result).
 
 Work goes to the current stream of the tensors' device and nothing waits for it.  A plan or tensor that another stream uses is recorded there by its owner, as
-everywhere in torch (plan.offsets.record_stream).  A call may be captured into a graph (a backward pass through torch.autograd.grad, as nothing may be left to do
-on the leaves' own stream).  torch.jit.trace and make_fx record torch's own operations only: an operator raises under them, and for tensors that wrap others.
+everywhere in torch (plan.offsets.record_stream).  A call may be captured into a graph; a backward pass through torch.autograd.grad, as nothing may be left to do
+on the leaves' own stream, and with no autograd graph from outside of the capture alive on the same leaves, whose stream torch would join with the capture.
+torch.jit.trace and make_fx record torch's own operations only: an operator raises under them, and for tensors that wrap others.
 
 The gradients of sort_rows, combine_rows and expert_linear come through torch.autograd, first order and in reverse (forward-mode derivatives raise).  Every
 operator gives the same bits for the same inputs.
